@@ -5,6 +5,7 @@
 #include <pybind11/stl.h>
 
 #include "../hip/hip_api.h"
+#include "../hip/mx.h"
 
 namespace py = pybind11;
 using namespace gpumon_hip;
@@ -42,6 +43,43 @@ PYBIND11_MODULE(_hip, m) {
                         static_cast<float*>(P(c)), s, n, blocks, P(stream));
   }, py::arg("dev"), py::arg("a"), py::arg("b"), py::arg("c"), py::arg("s"), py::arg("n"),
      py::arg("blocks") = 4096, py::arg("stream") = 0);
+
+  // MXFP4 operators (mx.h; on tensors: gpumon.ops.mx)
+  m.def("mx_quantize", [](int dev, uintptr_t x, const std::string& dtype, int64_t rows, int64_t k, int64_t stride,
+                          bool by_column, uintptr_t codes, uintptr_t scales, uintptr_t stream) {
+    launch_mx_quantize(dev, P(x), dtype, rows, k, stride, by_column, P(codes), P(scales), P(stream));
+  }, py::arg("dev"), py::arg("x"), py::arg("dtype"), py::arg("rows"), py::arg("k"), py::arg("stride"),
+     py::arg("by_column"), py::arg("codes"), py::arg("scales"), py::arg("stream") = 0);
+  m.def("mx_quantize_both", [](int dev, uintptr_t x, const std::string& dtype, int64_t rows, int64_t k, int64_t stride,
+                               uintptr_t row_codes, uintptr_t row_scales, uintptr_t col_codes, uintptr_t col_scales,
+                               uintptr_t stream) {
+    launch_mx_quantize_both(dev, P(x), dtype, rows, k, stride, P(row_codes), P(row_scales), P(col_codes),
+                            P(col_scales), P(stream));
+  }, py::arg("dev"), py::arg("x"), py::arg("dtype"), py::arg("rows"), py::arg("k"), py::arg("stride"),
+     py::arg("row_codes"), py::arg("row_scales"), py::arg("col_codes"), py::arg("col_scales"), py::arg("stream") = 0);
+  m.def("mx_dequantize", [](int dev, uintptr_t codes, uintptr_t scales, int64_t rows, int64_t k, uintptr_t out,
+                            const std::string& dtype, int64_t stride, uintptr_t stream) {
+    launch_mx_dequantize(dev, P(codes), P(scales), rows, k, P(out), dtype, stride, P(stream));
+  }, py::arg("dev"), py::arg("codes"), py::arg("scales"), py::arg("rows"), py::arg("k"), py::arg("out"),
+     py::arg("dtype"), py::arg("stride"), py::arg("stream") = 0);
+  m.def("mx_product_workspace", &mx_product_workspace, py::arg("dev"), py::arg("m"), py::arg("n"), py::arg("k"));
+  m.def("mx_product", [](int dev, uintptr_t a_codes, uintptr_t a_scales, uintptr_t b_codes, uintptr_t b_scales,
+                         int64_t m, int64_t n, int64_t k, uintptr_t c, const std::string& dtype, int64_t stride,
+                         uintptr_t workspace, size_t workspace_bytes, uintptr_t stream) {
+    launch_mx_product(dev, P(a_codes), P(a_scales), P(b_codes), P(b_scales), m, n, k, P(c), dtype, stride,
+                      P(workspace), workspace_bytes, P(stream));
+  }, py::arg("dev"), py::arg("a_codes"), py::arg("a_scales"), py::arg("b_codes"), py::arg("b_scales"), py::arg("m"),
+     py::arg("n"), py::arg("k"), py::arg("c"), py::arg("dtype"), py::arg("stride"), py::arg("workspace") = 0,
+     py::arg("workspace_bytes") = 0, py::arg("stream") = 0);
+  m.def("mx_linear_workspace", &mx_linear_workspace, py::arg("dev"), py::arg("m"), py::arg("n"), py::arg("k"));
+  m.def("mx_linear", [](int dev, uintptr_t x, const std::string& dtype, int64_t x_stride, uintptr_t w_codes,
+                        uintptr_t w_scales, int64_t m, int64_t n, int64_t k, uintptr_t y, int64_t y_stride,
+                        uintptr_t workspace, size_t workspace_bytes, uintptr_t stream) {
+    launch_mx_linear(dev, P(x), dtype, x_stride, P(w_codes), P(w_scales), m, n, k, P(y), y_stride, P(workspace),
+                     workspace_bytes, P(stream));
+  }, py::arg("dev"), py::arg("x"), py::arg("dtype"), py::arg("x_stride"), py::arg("w_codes"), py::arg("w_scales"),
+     py::arg("m"), py::arg("n"), py::arg("k"), py::arg("y"), py::arg("y_stride"), py::arg("workspace") = 0,
+     py::arg("workspace_bytes") = 0, py::arg("stream") = 0);
 
   py::class_<LoadGen>(m, "LoadGen")
       .def(py::init([](int dev, std::string kind, double duty, size_t hbm_bytes, int mfma_iters, int shape,

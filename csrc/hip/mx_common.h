@@ -1,0 +1,154 @@
+// What the MXFP4 kernels share: element types, the block's scale and codes, argument checks.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <stdexcept>
+#include <string>
+
+#include "hip_api.h"
+#include "mx.h"
+
+namespace gpumon_hip {
+namespace mx {
+
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+
+// The conversions of gfx950 divide (multiply) by the scale's power of two exactly, round halves to
+// even and saturate at 6, for every scale byte 0..254 including 2^-127, and read 255 as NaN; checked
+// over all 16-bit inputs times all scales against the definition.
+__device__ __forceinline__ float scale_of(unsigned byte) { return __builtin_bit_cast(float, byte << 23); }
+
+// Scale byte of a block from the bits of its largest magnitude as an f32 (magnitudes order like their
+// bits, and infinities and NaN come out on top): floor(log2) is the exponent field - 127, subnormals
+// end at the clamp.
+__device__ __forceinline__ unsigned scale_byte(unsigned amax_bits) {
+  const unsigned e = amax_bits >> 23;
+  return e == 255 ? 255u : e > 2 ? e - 2 : 0u;
+}
+
+template <typename T>
+struct Elem;
+template <>
+struct Elem<__bf16> {
+  static constexpr int kPerWord = 2;
+  using Word = unsigned;  // two elements
+  __device__ static unsigned amax(unsigned m, unsigned w) {  // running magnitudes, per half
+    return __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(u16x2, m),
+                                                                  __builtin_bit_cast(u16x2, w & 0x7fff7fffu)));
+  }
+  __device__ static unsigned amax_f32(unsigned m) { return max(m & 0xffff0000u, m << 16); }
+  template <int SEL>
+  __device__ static unsigned cvt(unsigned old, const unsigned* w, float s) {
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(old, __builtin_bit_cast(bf16x2, w[0]), s, SEL);
+  }
+  __device__ static __bf16 from_f32(float v) { return static_cast<__bf16>(v); }
+};
+template <>
+struct Elem<_Float16> {
+  static constexpr int kPerWord = 2;
+  using Word = unsigned;
+  __device__ static unsigned amax(unsigned m, unsigned w) { return Elem<__bf16>::amax(m, w); }
+  __device__ static unsigned amax_f32(unsigned m) {
+    const unsigned h = max(m >> 16, m & 0xffffu);  // an infinity or NaN converts to one
+    return __builtin_bit_cast(unsigned, static_cast<float>(__builtin_bit_cast(_Float16, static_cast<unsigned short>(h))));
+  }
+  template <int SEL>
+  __device__ static unsigned cvt(unsigned old, const unsigned* w, float s) {
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(old, __builtin_bit_cast(f16x2, w[0]), s, SEL);
+  }
+  __device__ static _Float16 from_f32(float v) { return static_cast<_Float16>(v); }
+};
+template <>
+struct Elem<float> {
+  static constexpr int kPerWord = 1;
+  using Word = unsigned;
+  __device__ static unsigned amax(unsigned m, unsigned w) { return max(m, w & 0x7fffffffu); }
+  __device__ static unsigned amax_f32(unsigned m) { return m; }
+  template <int SEL>
+  __device__ static unsigned cvt(unsigned old, const unsigned* w, float s) {
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(old, __builtin_bit_cast(float, w[0]),
+                                                    __builtin_bit_cast(float, w[1]), s, SEL);
+  }
+  __device__ static float from_f32(float v) { return v; }
+};
+
+// Eight elements to one word of codes. `w`: the elements' words (4 of 16-bit types, 8 of f32).
+template <typename T>
+__device__ __forceinline__ unsigned codes8(const unsigned* w, float s) {
+  constexpr int P = 2 / Elem<T>::kPerWord;  // words a pair
+  unsigned c = 0;
+  c = Elem<T>::template cvt<0>(c, w, s);
+  c = Elem<T>::template cvt<1>(c, w + P, s);
+  c = Elem<T>::template cvt<2>(c, w + 2 * P, s);
+  c = Elem<T>::template cvt<3>(c, w + 3 * P, s);
+  return c;
+}
+
+template <int CTRL>
+__device__ __forceinline__ unsigned dpp(unsigned v) {  // another lane's v, within rows of 16 lanes
+  return static_cast<unsigned>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, 0xf, 0xf, true));
+}
+constexpr int kXor1 = 0xB1, kXor2 = 0x4E, kRor4 = 0x124, kRor8 = 0x128;
+
+// x / d for x < 2^31 as a multiplication: m = floor(2^(31 + l) / d) + 1 with 2^l >= d errs by less
+// than one part in 2^31 of the quotient, so the floor is exact.
+struct Div {
+  unsigned d, m;
+  int s;
+  explicit Div(unsigned div) : d(div), m(0), s(0) {
+    int l = 0;
+    while ((1ull << l) < div) ++l;
+    m = static_cast<unsigned>((1ull << (31 + l)) / div + 1);
+    s = l - 1;
+  }
+  __device__ __forceinline__ unsigned quot(unsigned x) const { return d == 1 ? x : __umulhi(x, m) >> s; }
+};
+
+// ---- host ------------------------------------------------------------------------------------
+// Keeps the calling thread's current device.
+class OnDevice {
+ public:
+  explicit OnDevice(int dev) {
+    check(hipGetDevice(&old_), "hipGetDevice");
+    if (old_ != dev) check(hipSetDevice(dev), "hipSetDevice");
+    dev_ = dev;
+  }
+  ~OnDevice() {
+    if (old_ != dev_) (void)hipSetDevice(old_);
+  }
+
+ private:
+  int old_ = 0, dev_ = 0;
+};
+
+inline void require(bool ok, const char* what) {
+  if (!ok) throw std::invalid_argument(what);
+}
+inline bool aligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
+
+enum class Type { bf16, f16, f32 };
+inline Type type_of(const std::string& s, const char* what) {
+  if (s == "bf16") return Type::bf16;
+  if (s == "f16") return Type::f16;
+  if (s == "f32") return Type::f32;
+  throw std::invalid_argument(what);
+}
+inline int size_of(Type t) { return t == Type::f32 ? 4 : 2; }
+template <typename F>
+void with_type(Type t, F f) {  // f(T{})
+  if (t == Type::bf16) f(__bf16{});
+  else if (t == Type::f16) f(_Float16{});
+  else f(float{});
+}
+
+}  // namespace mx
+}  // namespace gpumon_hip

@@ -1,0 +1,267 @@
+"""MXFP4 operators on GPU tensors: quantisation, product, linear layer and its training step.
+
+What a node that serves or trains in 4 bits runs on the matrix path that
+``gpu_mfma_tflops{dtype="f6f4"}`` counts, as hand-written gfx950 kernels (``csrc/hip/mx_quant.hip``,
+``csrc/hip/mx_product.hip``; format and layout: ``csrc/hip/mx.h``). ``gpumon load --kind mxlinear``
+drives the card with them.
+
+An MXFP4 matrix holds 32 consecutive elements of a row as 4-bit numbers (0, 0.5, 1, 1.5, 2, 3, 4, 6
+and their negatives) times one power of two, ``2^(floor(log2 amax) - 2)``; elements are rounded to
+nearest, halves to the even code, and end at 6. A block with a NaN or an infinity stands for NaN.
+
+* :func:`quantize` / :func:`quantize_both` / :func:`dequantize` — to the format and back.
+* :func:`matmul` — ``a @ b.T`` of two quantised matrices, f32 sums.
+* :func:`linear` — unquantised rows on quantised weights (serving: single tokens to prompts).
+* :func:`linear_train` / :func:`linear_grad` — the layer's training step, all three products in 4 bits.
+
+Tensors are bf16, f16 or f32 on one GPU; work goes to that device's current torch stream and can be
+captured into a graph (workspaces come from torch's allocator, so each graph has its own). Results
+carry no autograd graph: :func:`linear_grad` is the backward pass. Errors of arguments are
+``ValueError`` / ``TypeError``, before anything is launched.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from .._native import hip
+
+DTYPES = {torch.bfloat16: "bf16", torch.float16: "f16", torch.float32: "f32"}
+BLOCK = 32
+_QUAD = 128  # rows are filled up with zeros to whole quads of blocks
+
+
+def _stream(device) -> int:
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _check(t, name: str, ndim=None):
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"mx: {name} must be a tensor, not {type(t).__name__}")
+    if not t.is_cuda:
+        raise ValueError(f"mx: {name} must be on a GPU, it is on {t.device}")
+    if t.dtype not in DTYPES:
+        raise TypeError(f"mx: {name} is {t.dtype}: one of bfloat16, float16, float32")
+    if ndim is not None and t.dim() != ndim:
+        raise ValueError(f"mx: {name} has {t.dim()} dimensions, expected {ndim}")
+
+
+def _check_dtype(dtype):
+    if dtype not in DTYPES:
+        raise TypeError(f"mx: dtype {dtype}: one of bfloat16, float16, float32")
+
+
+def _rows(x):
+    """x (2-D) with its elements next to each other along a row and no overlapping rows (else a copy)."""
+    return x if (x.stride(1) == 1 or x.shape[1] == 1) and x.stride(0) >= x.shape[1] else x.contiguous()
+
+
+def _row_stride(x) -> int:
+    return max(x.stride(0), x.shape[1])
+
+
+class MxTensor:
+    """A quantised matrix, ``rows`` x ``k`` with blocks along ``k``: ``codes`` [rows, quads * 64] uint8
+    and ``scales`` [quads, rows, 4] uint8 (quads = ceil(k / 128)), views of one buffer."""
+
+    __slots__ = ("buf", "rows", "k", "quads", "device", "_codes", "_scales")
+
+    def __init__(self, rows: int, k: int, device):
+        if rows < 0 or k < 1:
+            raise ValueError(f"mx: a quantised matrix needs rows >= 0 and k >= 1, not {rows} x {k}")
+        self.rows, self.k, self.quads = rows, k, -(-k // _QUAD)
+        self.buf = torch.empty(rows * self.quads * 68, dtype=torch.uint8, device=device)
+        self.device = self.buf.device
+        self._codes = self.buf.data_ptr()
+        self._scales = self._codes + rows * self.quads * 64
+
+    @property
+    def shape(self):
+        return (self.rows, self.k)
+
+    @property
+    def codes(self):
+        return self.buf[:self.rows * self.quads * 64].view(self.rows, self.quads * 64)
+
+    @property
+    def scales(self):
+        return self.buf[self.rows * self.quads * 64:].view(self.quads, self.rows, 4)
+
+    @staticmethod
+    def pack(codes, scales, k: int) -> "MxTensor":
+        """From row-major parts on a GPU: codes [rows, ceil(k/32)*16] uint8 (the even element in the low
+        nibble), scales [rows, ceil(k/32)] uint8 (exponent + 127; 255: NaN). Elements past k are ignored."""
+        blocks = -(-k // BLOCK)
+        for t, name, width in ((codes, "codes", blocks * 16), (scales, "scales", blocks)):
+            if not isinstance(t, torch.Tensor) or t.dtype != torch.uint8:
+                raise TypeError(f"mx: {name} must be a uint8 tensor")
+            if not t.is_cuda:
+                raise ValueError(f"mx: {name} must be on a GPU, it is on {t.device}")
+            if t.dim() != 2 or t.shape[1] != width or t.shape[0] != codes.shape[0]:
+                raise ValueError(f"mx: {name} is {tuple(t.shape)}, expected ({codes.shape[0]}, {width}) for k = {k}")
+        if codes.device != scales.device:
+            raise ValueError(f"mx: codes are on {codes.device}, scales on {scales.device}")
+        q = MxTensor(codes.shape[0], k, codes.device)
+        q.buf.zero_()
+        q.codes[:, :(k + 1) // 2] = codes[:, :(k + 1) // 2]
+        if k % 2:
+            q.codes[:, k // 2] &= 15
+        pad = scales.new_zeros(q.rows, q.quads * 4)
+        pad[:, :blocks] = scales
+        q.scales.copy_(pad.view(q.rows, q.quads, 4).transpose(0, 1))
+        return q
+
+    def parts(self):
+        """(codes, scales) row-major, as :meth:`pack` takes them."""
+        blocks = -(-self.k // BLOCK)
+        scales = self.scales.transpose(0, 1).reshape(self.rows, self.quads * 4)
+        return self.codes[:, :blocks * 16].contiguous(), scales[:, :blocks].contiguous()
+
+    def __repr__(self):
+        return f"MxTensor({self.rows} x {self.k}, {self.device})"
+
+
+def _check_mx(q, name: str):
+    if not isinstance(q, MxTensor):
+        raise TypeError(f"mx: {name} must be an MxTensor, not {type(q).__name__}")
+
+
+def quantize(x, axis: int = 1) -> MxTensor:
+    """x [r, c] with blocks along its rows (``axis`` 1 or -1: r x c) or down its columns (``axis`` 0 or
+    -2: c x r, the transposed matrix, as a product that contracts over r takes it)."""
+    _check(x, "x", 2)
+    if axis not in (0, 1, -1, -2):
+        raise ValueError(f"mx: axis {axis}: 0 or 1")
+    down = axis in (0, -2)
+    if x.stride(0) == 1 and x.stride(1) >= x.shape[0] > 1:  # a transposed view: the other direction of its base
+        x, down = x.t(), not down
+    x = _rows(x)
+    r, c = x.shape
+    q = MxTensor(c, r, x.device) if down else MxTensor(r, c, x.device)
+    if q.rows:
+        hip().mx_quantize(x.device.index, x.data_ptr(), DTYPES[x.dtype], r, c, _row_stride(x), down, q._codes, q._scales,
+                          _stream(x.device))
+    return q
+
+
+def quantize_both(x):
+    """``(quantize(x, 1), quantize(x, 0))`` from one reading of x."""
+    _check(x, "x", 2)
+    swap = x.stride(0) == 1 and x.stride(1) >= x.shape[0] > 1
+    x = _rows(x.t() if swap else x)
+    r, c = x.shape
+    along, down = MxTensor(r, c, x.device), MxTensor(c, r, x.device)
+    hip().mx_quantize_both(x.device.index, x.data_ptr(), DTYPES[x.dtype], r, c, _row_stride(x), along._codes,
+                           along._scales, down._codes, down._scales, _stream(x.device))
+    return (down, along) if swap else (along, down)
+
+
+def dequantize(q: MxTensor, dtype=torch.float32):
+    """What q stands for, [rows, k]; exact in bf16 and f32, rounded in f16."""
+    _check_mx(q, "q")
+    _check_dtype(dtype)
+    out = torch.empty(q.rows, q.k, dtype=dtype, device=q.device)
+    if q.rows:
+        hip().mx_dequantize(q.device.index, q._codes, q._scales, q.rows, q.k, out.data_ptr(), DTYPES[dtype], q.k,
+                            _stream(q.device))
+    return out
+
+
+def matmul(a: MxTensor, b: MxTensor, dtype=torch.bfloat16):
+    """a [m, k] @ b [n, k].T in ``dtype``: sums in 32 bits, rounded once."""
+    _check_mx(a, "a")
+    _check_mx(b, "b")
+    _check_dtype(dtype)
+    if a.k != b.k:
+        raise ValueError(f"mx: a is {a.rows} x {a.k} and b {b.rows} x {b.k}: the second sizes differ")
+    if a.device != b.device:
+        raise ValueError(f"mx: a is on {a.device}, b on {b.device}")
+    c = torch.empty(a.rows, b.rows, dtype=dtype, device=a.device)
+    if c.numel():
+        h, dev = hip(), a.device.index
+        need = h.mx_product_workspace(dev, a.rows, b.rows, a.k)
+        ws = torch.empty(need, dtype=torch.uint8, device=a.device) if need else None
+        h.mx_product(dev, a._codes, a._scales, b._codes, b._scales, a.rows, b.rows, a.k, c.data_ptr(), DTYPES[dtype],
+                     b.rows, ws.data_ptr() if need else 0, need, _stream(a.device))
+    return c
+
+
+def linear(x, w: MxTensor):
+    """x [..., k] on weights w (n x k): x quantised along k, times w.T; [..., n] in x's type."""
+    _check(x, "x")
+    _check_mx(w, "w")
+    if x.dim() < 1 or x.shape[-1] != w.k:
+        raise ValueError(f"mx: x is {tuple(x.shape)}, its last size must be the weights' k = {w.k}")
+    if x.device != w.device:
+        raise ValueError(f"mx: x is on {x.device}, w on {w.device}")
+    x2 = x if x.dim() == 2 else x.reshape(-1, w.k)
+    x2 = _rows(x2)
+    m, n = x2.shape[0], w.rows
+    y = torch.empty(*x.shape[:-1], n, dtype=x.dtype, device=x.device)
+    if y.numel():
+        h, dev = hip(), x.device.index
+        need = h.mx_linear_workspace(dev, m, n, w.k)
+        ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+        h.mx_linear(dev, x2.data_ptr(), DTYPES[x.dtype], _row_stride(x2), w._codes, w._scales, m, n, w.k, y.data_ptr(),
+                    n, ws.data_ptr() if need else 0, need, _stream(x.device))
+    return y
+
+
+class LinearSaved:
+    """What :func:`linear_train` keeps for :func:`linear_grad`: x and w with blocks along the axes that
+    the gradients contract over."""
+
+    __slots__ = ("x", "w", "shape", "n", "dtype", "w_dtype", "device")
+
+
+def linear_train(x, w):
+    """Forward pass with x [..., k] and w [n, k] both quantised here: ``(y [..., n], saved)``."""
+    _check(x, "x")
+    _check(w, "w", 2)
+    if x.dim() < 1 or x.shape[-1] != w.shape[1]:
+        raise ValueError(f"mx: x is {tuple(x.shape)}, w {tuple(w.shape)}: the last sizes differ")
+    if x.device != w.device:
+        raise ValueError(f"mx: x is on {x.device}, w on {w.device}")
+    n, k = w.shape
+    if n < 1 or k < 1:
+        raise ValueError(f"mx: w is {tuple(w.shape)}: neither size may be 0")
+    saved = LinearSaved()
+    saved.shape, saved.n, saved.dtype, saved.w_dtype, saved.device = tuple(x.shape), n, x.dtype, w.dtype, x.device
+    x2 = x.reshape(-1, k)
+    wq, saved.w = quantize_both(w)
+    if x2.shape[0] == 0:
+        saved.x = None
+        return torch.empty(*x.shape[:-1], n, dtype=x.dtype, device=x.device), saved
+    xq, saved.x = quantize_both(x2)
+    return matmul(xq, wq, x.dtype).view(*x.shape[:-1], n), saved
+
+
+def linear_grad(dy, saved: LinearSaved, need_dx: bool = True, need_dw: bool = True):
+    """Backward pass: ``(dx, dw)`` in x's and w's type (None where not needed). Straight-through: the
+    gradients of the layer as if quantising were the identity, each product in 4 bits with dy
+    quantised along the axis that it contracts over."""
+    _check(dy, "dy")
+    if not isinstance(saved, LinearSaved):
+        raise TypeError(f"mx: saved must come from linear_train, not {type(saved).__name__}")
+    if tuple(dy.shape) != saved.shape[:-1] + (saved.n,):
+        raise ValueError(f"mx: dy is {tuple(dy.shape)}, expected {saved.shape[:-1] + (saved.n,)}")
+    if dy.dtype != saved.dtype:
+        raise TypeError(f"mx: dy is {dy.dtype}, the layer's output {saved.dtype}")
+    if dy.device != saved.device:
+        raise ValueError(f"mx: dy is on {dy.device}, the layer on {saved.device}")
+    k = saved.shape[-1]
+    if saved.x is None:  # no rows
+        return (torch.empty(saved.shape, dtype=saved.dtype, device=saved.device) if need_dx else None,
+                torch.zeros(saved.n, k, dtype=saved.w_dtype, device=saved.device) if need_dw else None)
+    d2 = dy.reshape(-1, saved.n)
+    dx = dw = None
+    if need_dx and need_dw:
+        along, down = quantize_both(d2)
+    else:
+        along = quantize(d2, 1) if need_dx else None
+        down = quantize(d2, 0) if need_dw else None
+    if need_dx:
+        dx = matmul(along, saved.w, saved.dtype).view(saved.shape)
+    if need_dw:
+        dw = matmul(down, saved.x, saved.w_dtype)
+    return dx, dw

@@ -1,0 +1,96 @@
+"""What the MXFP4 operators refuse, checked without a GPU: every refusal comes before any GPU call."""
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+
+@pytest.fixture(scope="module")
+def mx():
+    from gpumon.ops import mx as m
+
+    return m
+
+
+@pytest.fixture(scope="module")
+def H():
+    from gpumon import hip
+
+    return hip()
+
+
+def test_tensors_on_the_cpu_and_other_types_are_refused(mx):
+    x = torch.zeros(4, 32)
+    for f in (mx.quantize, mx.quantize_both, lambda t: mx.linear(t, None), lambda t: mx.linear_train(t, t),
+              lambda t: mx.linear_grad(t, None)):
+        with pytest.raises(ValueError, match="on a GPU"):
+            f(x)
+        with pytest.raises(TypeError, match="tensor"):
+            f([1.0])
+    for f in (lambda: mx.matmul(x, x), lambda: mx.dequantize(x)):
+        with pytest.raises(TypeError, match="MxTensor"):
+            f()
+    with pytest.raises(TypeError, match="uint8"):
+        mx.MxTensor.pack(x, x, 32)
+    u = torch.zeros(4, 16, dtype=torch.uint8)
+    with pytest.raises(ValueError, match="on a GPU"):
+        mx.MxTensor.pack(u, u, 32)
+    for rows, k in ((-1, 5), (3, 0)):
+        with pytest.raises(ValueError, match="rows >= 0 and k >= 1"):
+            mx.MxTensor(rows, k, "cpu")
+
+
+def test_products_of_other_sizes_are_refused(mx):
+    a, b = mx.MxTensor(3, 64, "cpu"), mx.MxTensor(5, 65, "cpu")
+    with pytest.raises(ValueError, match="second sizes differ"):
+        mx.matmul(a, b)
+    with pytest.raises(TypeError, match="dtype"):
+        mx.matmul(a, a, torch.float64)
+    with pytest.raises(TypeError, match="dtype"):
+        mx.dequantize(a, torch.int32)
+
+
+P = 1 << 20  # an aligned address that nothing here reaches
+
+
+@pytest.mark.parametrize("over,match", [
+    ({"dtype": "f64"}, "dtype"), ({"rows": -1}, "rows"), ({"k": 0}, "k >= 1"), ({"stride": 31}, "stride"),
+    ({"rows": 1 << 31}, "2\\^31"), ({"rows": 1 << 20, "k": 1 << 20, "stride": 1 << 20}, "2\\^31"), ({"x": 0}, "null"),
+    ({"codes": 0}, "null"), ({"scales": 0}, "null"), ({"x": P + 1}, "aligned"), ({"codes": P + 8}, "aligned"),
+    ({"scales": P + 2}, "aligned")])
+def test_native_quantize_refuses(H, over, match):
+    ok = dict(dev=0, x=P, dtype="bf16", rows=4, k=32, stride=32, by_column=False, codes=P, scales=P)
+    with pytest.raises(ValueError, match=match):
+        H.mx_quantize(**{**ok, **over})
+    both = {**ok, **over}
+    both.pop("by_column")
+    codes, scales = both.pop("codes"), both.pop("scales")
+    with pytest.raises(ValueError, match=match):
+        H.mx_quantize_both(row_codes=codes, row_scales=scales, col_codes=codes, col_scales=scales, **both)
+    back = {**ok, **over}
+    back.pop("by_column")
+    with pytest.raises(ValueError, match=match):
+        H.mx_dequantize(out=back.pop("x"), **back)
+
+
+def test_native_quantize_by_column_refuses_no_rows(H):
+    with pytest.raises(ValueError, match="rows"):
+        H.mx_quantize(0, P, "bf16", 0, 32, 32, True, P, P)
+
+
+@pytest.mark.parametrize("over,match", [
+    ({"dtype": "f64"}, "dtype"), ({"m": -1}, "m and n"), ({"n": -1}, "m and n"), ({"k": 0}, "k >= 1"),
+    ({"stride": 47}, "stride"), ({"m": 1 << 31}, "beyond"), ({"n": 1 << 20, "k": 1 << 20, "stride": 1 << 20}, "beyond"),
+    ({"m": 1 << 30, "n": 1 << 30, "stride": 1 << 30}, "beyond"), ({"a_codes": 0}, "null"), ({"b_scales": 0}, "null"),
+    ({"c": 0}, "null"), ({"a_codes": P + 4}, "aligned"), ({"b_scales": P + 1}, "aligned"), ({"c": P + 1}, "aligned")])
+def test_native_product_refuses(H, over, match):
+    ok = dict(dev=0, a_codes=P, a_scales=P, b_codes=P, b_scales=P, m=4, n=48, k=64, c=P, dtype="bf16", stride=48)
+    with pytest.raises(ValueError, match=match):
+        H.mx_product(**{**ok, **over})
+
+
+def test_native_linear_refuses_a_small_workspace(H):
+    need = H.mx_linear_workspace(0, 300, 400, 500)
+    assert need > 0
+    with pytest.raises(ValueError, match="workspace"):
+        H.mx_linear(0, P, "bf16", 500, P, P, 300, 400, 500, P, 400, P, need - 1)
