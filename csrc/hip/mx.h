@@ -7,11 +7,14 @@
 //     q_i = x_i / 2^E rounded to the grid, halves to the even code, beyond 6 to 6;
 // a NaN or an infinity in the block: byte 255. Dividing by 2^E is exact, so every code is determined.
 //
-// Layout. k is filled up with zeros to whole "quads" of 128 elements, kq = ceil(k / 128):
-//     codes  [rows][kq * 64] bytes, the even element in the low nibble;
-//     scales [kq][rows] 32-bit words, byte b = block b of that quad of that row.
-// One lane's operand of v_mfma_scale_f32_16x16x128_f8f6f4 is one block (16 bytes of codes, one scale
-// byte), and the 16 rows that 16 lanes hold have their scale words next to each other.
+// Layout. Rows are filled up to blocks of 16 and k with zeros to quads of 128 elements (4 scale blocks):
+//     codes  [row block][quad][4 blocks][16 rows][16 bytes], the even element in the low nibble;
+//     scales [row block][group of 4 quads][4 blocks][16 rows][4 quads] bytes, zeros past the last quad.
+// A lane's operand of v_mfma_scale_f32_16x16x128_f8f6f4 is one block of one row (lane l: row l & 15,
+// block l >> 4), so a wave's operand is one "chunk" of 1 KiB in lane order, and the scale words of
+// four such steps are 256 bytes in lane order, the instruction picking the step's byte. Memory, LDS
+// and registers hold the same order: every transfer is contiguous, with no bank conflicts and no
+// shuffles.
 #pragma once
 
 #include <cstddef>
@@ -20,13 +23,19 @@
 
 namespace gpumon_hip {
 
-constexpr int64_t kMxBlock = 32, kMxQuad = 128;
-inline int64_t mx_quads(int64_t k) { return (k + kMxQuad - 1) / kMxQuad; }
+inline int64_t mx_quads(int64_t k) { return (k + 127) / 128; }
+inline int64_t mx_groups(int64_t k) { return (k + 511) / 512; }
+inline int64_t mx_row_blocks(int64_t rows) { return (rows + 15) / 16; }
 // bytes of codes and of scales
-inline int64_t mx_codes_bytes(int64_t rows, int64_t k) { return rows * mx_quads(k) * 64; }
-inline int64_t mx_scales_bytes(int64_t rows, int64_t k) { return rows * mx_quads(k) * 4; }
+inline int64_t mx_codes_bytes(int64_t rows, int64_t k) { return mx_row_blocks(rows) * mx_quads(k) * 1024; }
+inline int64_t mx_scales_bytes(int64_t rows, int64_t k) { return mx_row_blocks(rows) * mx_groups(k) * 256; }
+// Limits of the kernels' indexes and grids: 2^24 pieces of 16 rows x 512 elements (more than fits the
+// card in 16 bits an element); a product also has at most 2^28 pieces of 16 x 16 results.
+inline bool mx_fits(int64_t rows, int64_t k) {
+  return rows < (1ll << 28) && k < (1ll << 31) - 512 && mx_row_blocks(rows) * mx_groups(k) < (1ll << 24);
+}
 
-// All launches: dtype bf16 | f16 | f32; strides in elements; codes 16-byte, scales 4-byte aligned.
+// All launches: dtype bf16 | f16 | f32; strides in elements; codes and scales 16-byte aligned.
 // They throw std::invalid_argument before anything is launched, keep the calling thread's current
 // device, and need no synchronisation: they can be recorded into a graph.
 

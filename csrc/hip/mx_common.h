@@ -5,6 +5,7 @@
 
 #include <stdexcept>
 #include <string>
+#include <type_traits>
 
 #include "hip_api.h"
 #include "mx.h"
@@ -97,7 +98,7 @@ template <int CTRL>
 __device__ __forceinline__ unsigned dpp(unsigned v) {  // another lane's v, within rows of 16 lanes
   return static_cast<unsigned>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, 0xf, 0xf, true));
 }
-constexpr int kXor1 = 0xB1, kXor2 = 0x4E, kRor4 = 0x124, kRor8 = 0x128;
+constexpr int kXor1 = 0xB1, kXor2 = 0x4E;
 
 // x / d for x < 2^31 as a multiplication: m = floor(2^(31 + l) / d) + 1 with 2^l >= d errs by less
 // than one part in 2^31 of the quotient, so the floor is exact.

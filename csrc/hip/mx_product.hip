@@ -5,59 +5,165 @@ namespace gpumon_hip {
 namespace mx {
 namespace {
 
-// One wave's 16x16x128 step. Operand fragments: lane l holds row l & 15, block l >> 4 of the quad
-// (16 bytes), its scale in byte 0; D: lane l holds columns-of-B row l & 15 and rows-of-A 4 (l >> 4) + i.
+typedef __attribute__((address_space(3))) void LdsVoid;
+typedef const __attribute__((address_space(1))) void GlobalVoid;
+
+// One wave's 16x16x128 step on one chunk of either side; S picks the quad's byte of the scale words.
+// D: lane l holds row l & 15 of b's chunk and rows 4 (l >> 4) + i of a's.
+template <int S>
 __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c, unsigned sa, unsigned sb) {
   const i32x8 av = {(int)a[0], (int)a[1], (int)a[2], (int)a[3], 0, 0, 0, 0};
   const i32x8 bv = {(int)b[0], (int)b[1], (int)b[2], (int)b[3], 0, 0, 0, 0};
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, c, 4, 4, 0, (int)sa, 0, (int)sb);
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, c, 4, 4, S, (int)sa, S, (int)sb);
 }
 
-// 32 x 32 results a wave, operands straight from memory. b's rows take the instruction's A side, so
-// that a lane's four sums are neighbours in a row of c. Rows past the end read the last row instead,
-// and their sums are not stored.
-template <typename T>
-__global__ void __launch_bounds__(256) product_direct_kernel(const u32x4* __restrict__ ac, const unsigned* __restrict__ as,
-                                                             const u32x4* __restrict__ bc, const unsigned* __restrict__ bs,
-                                                             unsigned m, unsigned n, unsigned quads, T* __restrict__ c,
-                                                             int64_t stride, Div tiles_n) {
-  const unsigned lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
+// s_waitcnt with a vmcnt and, if lgkm0, lgkmcnt(0).
+constexpr int wait_imm(int vm, bool lgkm0) { return (vm & 15) | ((vm >> 4) << 14) | (7 << 4) | ((lgkm0 ? 0 : 15) << 8); }
+
+template <int S>
+using Int = std::integral_constant<int, S>;
+
+// 2 x 2 waves, FM x FN chunks of 16 x 16 results each.
+template <typename T, int FM, int FN>
+__global__ void __launch_bounds__(256, FM* FN > 32 ? 1 : 2)
+    product_tile_kernel(const char* __restrict__ ac, const char* __restrict__ as, const char* __restrict__ bc,
+                        const char* __restrict__ bs, unsigned m, unsigned n, unsigned quads, T* __restrict__ c,
+                        int64_t stride, Div tiles_n) {
+  constexpr int kChunks = 2 * (FM + FN), kLoads = kChunks / 4, kScaleLoads = kChunks >= 16 ? kChunks / 16 : 1;
+  constexpr int kStage = kChunks * 1024, kScales = kChunks * 256;
+  __shared__ __attribute__((aligned(16))) char lds[4 * kStage + 2 * kScales];
+  const unsigned lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const unsigned tm = tiles_n.quot(blockIdx.x), tn = blockIdx.x - tm * tiles_n.d;
-  const unsigned m0 = tm * 64 + (wave & 1) * 32, n0 = tn * 64 + (wave >> 1) * 32;
-  unsigned rm[2], rn[2];
-  for (int f = 0; f < 2; ++f) rm[f] = min(m0 + f * 16 + r, m - 1), rn[f] = min(n0 + f * 16 + r, n - 1);
-  f32x4 acc[2][2] = {};
-  for (unsigned q = 0; q < quads; ++q) {
-    u32x4 a[2], b[2];
-    unsigned sa[2], sb[2];
+  const unsigned rbm = (m + 15) / 16, rbn = (n + 15) / 16, groups = (quads + 3) / 4;
+  const unsigned wm = wave & 1, wn = wave >> 1;
+
+  // chunk `x` of the tile, a's 2 FM first; row blocks past the end read the last one instead, and what
+  // comes of them is not stored
+  auto row_block = [&](unsigned x) {
+    return x < 2 * FM ? min(tm * (2 * FM) + x, rbm - 1) : min(tn * (2 * FN) + x - 2 * FM, rbn - 1);
+  };
+  const char* src[kLoads];
 #pragma unroll
-    for (int f = 0; f < 2; ++f) {
-      a[f] = ac[(static_cast<size_t>(rm[f]) * quads + q) * 4 + g];
-      b[f] = bc[(static_cast<size_t>(rn[f]) * quads + q) * 4 + g];
-      sa[f] = as[static_cast<size_t>(q) * m + rm[f]] >> (8 * g);
-      sb[f] = bs[static_cast<size_t>(q) * n + rn[f]] >> (8 * g);
+  for (int i = 0; i < kLoads; ++i) {
+    const unsigned x = wave * kLoads + i;
+    src[i] = (x < 2 * FM ? ac : bc) + static_cast<size_t>(row_block(x)) * quads * 1024;
+  }
+  const char* ssrc[kScaleLoads];
+#pragma unroll
+  for (int i = 0; i < kScaleLoads; ++i) {
+    const unsigned x = ((wave * kScaleLoads + i) * 4 + (lane >> 4)) % kChunks;
+    ssrc[i] = (x < 2 * FM ? as : bs) + static_cast<size_t>(row_block(x)) * groups * 256 + (lane & 15) * 16;
+  }
+  auto load_stage = [&](unsigned t, int slot) {
+    const unsigned q = min(t, quads - 1);
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i)
+      __builtin_amdgcn_global_load_lds((GlobalVoid*)(src[i] + static_cast<size_t>(q) * 1024 + lane * 16),
+                                       (LdsVoid*)(lds + slot * kStage + (wave * kLoads + i) * 1024), 16, 0, 0);
+  };
+  auto load_scales = [&](unsigned g) {
+    const unsigned q = min(g, groups - 1);
+#pragma unroll
+    for (int i = 0; i < kScaleLoads; ++i)
+      __builtin_amdgcn_global_load_lds(
+          (GlobalVoid*)(ssrc[i] + static_cast<size_t>(q) * 256),
+          (LdsVoid*)(lds + 4 * kStage + (g & 1) * kScales + (wave * kScaleLoads + i) * 1024 % kScales), 16, 0, 0);
+  };
+
+  u32x4 fa[2][FM], fb[2][FN];
+  unsigned sa[FM], sb[FN], sa2[FM], sb2[FN];
+  f32x4 acc[FM][FN] = {};
+  auto read_stage = [&](int slot, u32x4* a, u32x4* b) {
+    const char* p = lds + slot * kStage + lane * 16;
+#pragma unroll
+    for (int i = 0; i < FM; ++i) a[i] = *reinterpret_cast<const u32x4*>(p + (wm * FM + i) * 1024);
+#pragma unroll
+    for (int j = 0; j < FN; ++j) b[j] = *reinterpret_cast<const u32x4*>(p + (2 * FM + wn * FN + j) * 1024);
+  };
+  auto read_scales = [&](unsigned g, unsigned* a, unsigned* b) {
+    const char* p = lds + 4 * kStage + (g & 1) * kScales + lane * 4;
+#pragma unroll
+    for (int i = 0; i < FM; ++i) a[i] = *reinterpret_cast<const unsigned*>(p + (wm * FM + i) * 256);
+#pragma unroll
+    for (int j = 0; j < FN; ++j) b[j] = *reinterpret_cast<const unsigned*>(p + (2 * FM + wn * FN + j) * 256);
+  };
+
+  load_scales(0);
+#pragma unroll
+  for (int t = 0; t < 4; ++t) load_stage(t, t);
+  __builtin_amdgcn_s_waitcnt(wait_imm(3 * kLoads, false));
+  __builtin_amdgcn_s_barrier();
+  read_scales(0, sa, sb);
+  read_stage(0, fa[0], fb[0]);
+
+  auto body = [&](unsigned g, auto step) {
+    constexpr int J = decltype(step)::value;
+    const unsigned t = g * 4 + J;
+    // stage t + 1 is here, for every wave, and every wave has read stage t
+    __builtin_amdgcn_s_waitcnt(wait_imm(2 * kLoads + (J == 1 || J == 2 ? kScaleLoads : 0), true));
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (J == 0) load_scales(g + 1);
+    load_stage(t + 4, J);
+    read_stage((J + 1) & 3, fa[(J + 1) & 1], fb[(J + 1) & 1]);
+    if constexpr (J == 3) read_scales(g + 1, sa2, sb2);
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+      for (int j = 0; j < FN; ++j)
+        acc[i][j] = mfma16<J>(fb[J & 1][j], fa[J & 1][i], acc[i][j], sb[j], sa[i]);
+    if constexpr (J == 3) {
+#pragma unroll
+      for (int i = 0; i < FM; ++i) sa[i] = sa2[i];
+#pragma unroll
+      for (int j = 0; j < FN; ++j) sb[j] = sb2[j];
     }
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) acc[i][j] = mfma16(b[j], a[i], acc[i][j], sb[j], sa[i]);
+    for (int i = 0; i < FM + FN; ++i) {  // one read of LDS, then its share of the matrix instructions
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, FM * FN / (FM + FN), 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  const unsigned whole = quads / 4, rest = quads & 3;
+  for (unsigned g = 0; g < whole; ++g) {
+    body(g, Int<0>{});
+    body(g, Int<1>{});
+    body(g, Int<2>{});
+    body(g, Int<3>{});
   }
+  if (rest > 0) body(whole, Int<0>{});
+  if (rest > 1) body(whole, Int<1>{});
+  if (rest > 2) body(whole, Int<2>{});
+  __builtin_amdgcn_s_waitcnt(wait_imm(0, true));  // nothing may arrive after the workgroup's memory is given back
+
+  const unsigned row0 = (tm * 2 + wm) * FM * 16 + (lane & 15), col0 = (tn * 2 + wn) * FN * 16 + (lane >> 4) * 4;
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int i = 0; i < FM; ++i) {
+    const unsigned row = row0 + i * 16;
+    if (row >= m) continue;
+    T* out = c + static_cast<int64_t>(row) * stride;
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int j = 0; j < FN; ++j) {
+      const unsigned col = col0 + j * 16;
+      T v[4];
 #pragma unroll
-      for (unsigned e = 0; e < 4; ++e) {
-        const unsigned row = m0 + i * 16 + r, col = n0 + j * 16 + g * 4 + e;
-        if (row < m && col < n) c[static_cast<int64_t>(row) * stride + col] = Elem<T>::from_f32(acc[i][j][e]);
+      for (int e = 0; e < 4; ++e) v[e] = Elem<T>::from_f32(acc[i][j][e]);
+      if (col + 4 <= n) {
+        __builtin_memcpy(out + col, v, sizeof(v));
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (col + e < n) out[col + e] = v[e];
       }
+    }
+  }
 }
 
 void check_product(int64_t m, int64_t n, int64_t k, int64_t stride) {
   require(m >= 0 && n >= 0 && k >= 1, "mx: m and n must be >= 0 and k >= 1");
-  require(m < (1ll << 31) && n < (1ll << 31) && k <= (1ll << 31) - 256 && m * mx_quads(k) < (1ll << 31) &&
-              n * mx_quads(k) < (1ll << 31) && ((m + 63) / 64) * ((n + 63) / 64) < (1ll << 31),
-          "mx: a product's sizes are beyond what its grid holds (2^31 quads of a side, 2^31 tiles of 64 x 64)");
+  require(mx_fits(m, k) && mx_fits(n, k) && ((m + 15) / 16) * ((n + 15) / 16) < (1ll << 28),
+          "mx: a product's sizes are beyond its limits (mx.h)");
   require(stride >= n || m <= 1, "mx: stride must be at least n");
 }
 
@@ -80,18 +186,23 @@ void launch_mx_product(int dev, const void* a_codes, const void* a_scales, const
   check_product(m, n, k, stride);
   if (m == 0 || n == 0) return;
   require(a_codes && a_scales && b_codes && b_scales && c, "mx_product: null pointer");
-  require(aligned(a_codes, 16) && aligned(b_codes, 16) && aligned(a_scales, 4) && aligned(b_scales, 4) &&
+  require(aligned(a_codes, 16) && aligned(b_codes, 16) && aligned(a_scales, 16) && aligned(b_scales, 16) &&
               aligned(c, size_of(t)),
-          "mx_product: codes aligned to 16, scales to 4 bytes, the result to its type");
+          "mx_product: codes and scales aligned to 16 bytes, the result to its type");
   OnDevice on(dev);
-  const unsigned tn = static_cast<unsigned>((n + 63) / 64), tm = static_cast<unsigned>((m + 63) / 64);
   with_type(t, [&](auto e) {
     using T = decltype(e);
-    hipLaunchKernelGGL(product_direct_kernel<T>, dim3(tm * tn), dim3(256), 0, static_cast<hipStream_t>(stream),
-                       static_cast<const u32x4*>(a_codes), static_cast<const unsigned*>(a_scales),
-                       static_cast<const u32x4*>(b_codes), static_cast<const unsigned*>(b_scales),
-                       static_cast<unsigned>(m), static_cast<unsigned>(n), static_cast<unsigned>(mx_quads(k)),
-                       static_cast<T*>(c), stride, Div(tn));
+    auto run = [&](auto kernel, int tile_m, int tile_n) {
+      const unsigned tn = static_cast<unsigned>((n + tile_n - 1) / tile_n), tm = static_cast<unsigned>((m + tile_m - 1) / tile_m);
+      hipLaunchKernelGGL(kernel, dim3(tm * tn), dim3(256), 0, static_cast<hipStream_t>(stream),
+                         static_cast<const char*>(a_codes), static_cast<const char*>(a_scales),
+                         static_cast<const char*>(b_codes), static_cast<const char*>(b_scales),
+                         static_cast<unsigned>(m), static_cast<unsigned>(n), static_cast<unsigned>(mx_quads(k)),
+                         static_cast<T*>(c), stride, Div(tn));
+    };
+    if (m > 1024 && n > 1024) run(product_tile_kernel<T, 8, 8>, 256, 256);
+    else if (m > 64 && n > 64) run(product_tile_kernel<T, 4, 4>, 128, 128);
+    else run(product_tile_kernel<T, 2, 2>, 64, 64);
   });
   check(hipGetLastError(), "mx_product");
 }

@@ -28,7 +28,6 @@ from .._native import hip
 
 DTYPES = {torch.bfloat16: "bf16", torch.float16: "f16", torch.float32: "f32"}
 BLOCK = 32
-_QUAD = 128  # rows are filled up with zeros to whole quads of blocks
 
 
 def _stream(device) -> int:
@@ -61,19 +60,23 @@ def _row_stride(x) -> int:
 
 
 class MxTensor:
-    """A quantised matrix, ``rows`` x ``k`` with blocks along ``k``: ``codes`` [rows, quads * 64] uint8
-    and ``scales`` [quads, rows, 4] uint8 (quads = ceil(k / 128)), views of one buffer."""
+    """A quantised matrix, ``rows`` x ``k`` with blocks along ``k``, in the kernels' order (views of one
+    buffer): ``codes`` [ceil(rows/16), ceil(k/128), 4 blocks, 16 rows, 16] uint8 and ``scales``
+    [ceil(rows/16), ceil(k/512), 4 blocks, 16 rows, 4 quads of blocks] uint8; zeros fill both up.
+    :meth:`parts` / :meth:`pack` are the row-major form."""
 
-    __slots__ = ("buf", "rows", "k", "quads", "device", "_codes", "_scales")
+    __slots__ = ("buf", "rows", "k", "device", "_codes", "_scales")
 
     def __init__(self, rows: int, k: int, device):
         if rows < 0 or k < 1:
             raise ValueError(f"mx: a quantised matrix needs rows >= 0 and k >= 1, not {rows} x {k}")
-        self.rows, self.k, self.quads = rows, k, -(-k // _QUAD)
-        self.buf = torch.empty(rows * self.quads * 68, dtype=torch.uint8, device=device)
+        rb = (rows + 15) // 16
+        codes = rb * ((k + 127) // 128) * 1024
+        self.rows, self.k = rows, k
+        self.buf = torch.empty(codes + rb * ((k + 511) // 512) * 256, dtype=torch.uint8, device=device)
         self.device = self.buf.device
         self._codes = self.buf.data_ptr()
-        self._scales = self._codes + rows * self.quads * 64
+        self._scales = self._codes + codes
 
     @property
     def shape(self):
@@ -81,11 +84,11 @@ class MxTensor:
 
     @property
     def codes(self):
-        return self.buf[:self.rows * self.quads * 64].view(self.rows, self.quads * 64)
+        return self.buf[:self._scales - self._codes].view(-(-self.rows // 16), -(-self.k // 128), 4, 16, 16)
 
     @property
     def scales(self):
-        return self.buf[self.rows * self.quads * 64:].view(self.quads, self.rows, 4)
+        return self.buf[self._scales - self._codes:].view(-(-self.rows // 16), -(-self.k // 512), 4, 16, 4)
 
     @staticmethod
     def pack(codes, scales, k: int) -> "MxTensor":
@@ -102,20 +105,23 @@ class MxTensor:
         if codes.device != scales.device:
             raise ValueError(f"mx: codes are on {codes.device}, scales on {scales.device}")
         q = MxTensor(codes.shape[0], k, codes.device)
-        q.buf.zero_()
-        q.codes[:, :(k + 1) // 2] = codes[:, :(k + 1) // 2]
+        rb, quads, groups = -(-q.rows // 16), -(-k // 128), -(-k // 512)
+        full = codes.new_zeros(rb * 16, quads * 64)
+        full[:q.rows, :(k + 1) // 2] = codes[:, :(k + 1) // 2]
         if k % 2:
-            q.codes[:, k // 2] &= 15
-        pad = scales.new_zeros(q.rows, q.quads * 4)
-        pad[:, :blocks] = scales
-        q.scales.copy_(pad.view(q.rows, q.quads, 4).transpose(0, 1))
+            full[:, k // 2] &= 15
+        q.codes.copy_(full.view(rb, 16, quads, 4, 16).permute(0, 2, 3, 1, 4))
+        full = scales.new_zeros(rb * 16, groups * 16)
+        full[:q.rows, :blocks] = scales
+        q.scales.copy_(full.view(rb, 16, groups, 4, 4).permute(0, 2, 4, 1, 3))
         return q
 
     def parts(self):
         """(codes, scales) row-major, as :meth:`pack` takes them."""
-        blocks = -(-self.k // BLOCK)
-        scales = self.scales.transpose(0, 1).reshape(self.rows, self.quads * 4)
-        return self.codes[:, :blocks * 16].contiguous(), scales[:, :blocks].contiguous()
+        blocks, r16 = -(-self.k // BLOCK), -(-self.rows // 16) * 16
+        codes = self.codes.permute(0, 3, 1, 2, 4).reshape(r16, -1)[:self.rows, :blocks * 16]
+        scales = self.scales.permute(0, 3, 1, 4, 2).reshape(r16, -1)[:self.rows, :blocks]
+        return codes.contiguous(), scales.contiguous()
 
     def __repr__(self):
         return f"MxTensor({self.rows} x {self.k}, {self.device})"

@@ -55,7 +55,7 @@ P = 1 << 20  # an aligned address that nothing here reaches
 
 @pytest.mark.parametrize("over,match", [
     ({"dtype": "f64"}, "dtype"), ({"rows": -1}, "rows"), ({"k": 0}, "k >= 1"), ({"stride": 31}, "stride"),
-    ({"rows": 1 << 31}, "2\\^31"), ({"rows": 1 << 20, "k": 1 << 20, "stride": 1 << 20}, "2\\^31"), ({"x": 0}, "null"),
+    ({"rows": 1 << 31}, "limits"), ({"rows": 1 << 20, "k": 1 << 20, "stride": 1 << 20}, "limits"), ({"x": 0}, "null"),
     ({"codes": 0}, "null"), ({"scales": 0}, "null"), ({"x": P + 1}, "aligned"), ({"codes": P + 8}, "aligned"),
     ({"scales": P + 2}, "aligned")])
 def test_native_quantize_refuses(H, over, match):
@@ -80,8 +80,8 @@ def test_native_quantize_by_column_refuses_no_rows(H):
 
 @pytest.mark.parametrize("over,match", [
     ({"dtype": "f64"}, "dtype"), ({"m": -1}, "m and n"), ({"n": -1}, "m and n"), ({"k": 0}, "k >= 1"),
-    ({"stride": 47}, "stride"), ({"m": 1 << 31}, "beyond"), ({"n": 1 << 20, "k": 1 << 20, "stride": 1 << 20}, "beyond"),
-    ({"m": 1 << 30, "n": 1 << 30, "stride": 1 << 30}, "beyond"), ({"a_codes": 0}, "null"), ({"b_scales": 0}, "null"),
+    ({"stride": 47}, "stride"), ({"m": 1 << 31}, "limits"), ({"n": 1 << 20, "k": 1 << 20, "stride": 1 << 20}, "limits"),
+    ({"m": 1 << 30, "n": 1 << 30, "stride": 1 << 30}, "limits"), ({"a_codes": 0}, "null"), ({"b_scales": 0}, "null"),
     ({"c": 0}, "null"), ({"a_codes": P + 4}, "aligned"), ({"b_scales": P + 1}, "aligned"), ({"c": P + 1}, "aligned")])
 def test_native_product_refuses(H, over, match):
     ok = dict(dev=0, a_codes=P, a_scales=P, b_codes=P, b_scales=P, m=4, n=48, k=64, c=P, dtype="bf16", stride=48)
