@@ -94,6 +94,21 @@ __device__ __forceinline__ unsigned codes8(const unsigned* w, float s) {
   return c;
 }
 
+// Eight elements of a row from column k0 on as words, zeros from column k on. Rows start where the
+// caller's stride puts them, so the 16 bytes need not be aligned (one unaligned load).
+template <typename T>
+__device__ __forceinline__ void load8(const T* __restrict__ row, int k0, int k, unsigned* w) {
+  constexpr int N = 8 / Elem<T>::kPerWord;
+  if (k0 + 8 <= k) {
+    __builtin_memcpy(w, row + k0, N * 4);
+  } else {
+    T v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = k0 + j < k ? row[k0 + j] : T{};
+    __builtin_memcpy(w, v, N * 4);
+  }
+}
+
 template <int CTRL>
 __device__ __forceinline__ unsigned dpp(unsigned v) {  // another lane's v, within rows of 16 lanes
   return static_cast<unsigned>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, 0xf, 0xf, true));

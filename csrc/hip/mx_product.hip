@@ -160,6 +160,167 @@ __global__ void __launch_bounds__(256, FM* FN > 32 ? 1 : 2)
   }
 }
 
+// ---- few rows ----------------------------------------------------------------------------------
+// x has at most 16 FM rows: the weights' bytes are the work. A workgroup takes R row blocks of b (16 R
+// results a row of x), its waves whole groups of quads in turn, straight from memory to registers,
+// U groups a wave in flight; the waves' sums meet in LDS in a fixed order. Sources of x: rows
+// quantised before, or plain rows that each wave quantises for its own groups.
+constexpr int kWaves = 8;
+
+struct QuantizedRows {
+  const char* codes;
+  const char* scales;
+  unsigned quads, groups, row_blocks;
+  struct Raw {};
+  static constexpr int kLds = 16;
+  template <int FM, bool FULL>
+  __device__ __forceinline__ void load(unsigned g, unsigned nq, unsigned lane, Raw&, u32x4 (&x)[4][FM], unsigned (&sx)[FM]) const {
+#pragma unroll
+    for (int f = 0; f < FM; ++f) {
+      const unsigned rb = min(static_cast<unsigned>(f), row_blocks - 1);
+      sx[f] = *reinterpret_cast<const unsigned*>(scales + (static_cast<size_t>(rb) * groups + g) * 256 + lane * 4);
+#pragma unroll
+      for (unsigned q = 0; q < 4; ++q)
+        if (FULL || q < nq)
+          x[q][f] = *reinterpret_cast<const u32x4*>(codes + (static_cast<size_t>(rb) * quads + g * 4 + q) * 1024 + lane * 16);
+        else
+          x[q][f] = u32x4{0, 0, 0, 0};
+    }
+  }
+  template <int FM>
+  __device__ __forceinline__ void finish(const Raw&, unsigned, char*, u32x4 (&)[4][FM], unsigned (&)[FM]) const {}
+};
+
+// Up to ROWS plain rows (ROWS <= 16): eight elements a lane of one row after the other, 16 lanes a quad,
+// as the quantising kernel does; the codes change lanes in the wave's own piece of LDS. Rows of the
+// operand from ROWS on repeat the last one.
+template <typename X, int ROWS>
+struct PlainRows {
+  const X* x;
+  int64_t stride;
+  unsigned m;
+  int k;
+  static constexpr int kWords = 8 / Elem<X>::kPerWord;
+  struct Raw {
+    unsigned w[ROWS][kWords];
+  };
+  static constexpr int kLds = ROWS * 256 + 64 * ROWS;
+  template <int FM, bool FULL>
+  __device__ __forceinline__ void load(unsigned g, unsigned, unsigned lane, Raw& raw, u32x4 (&)[4][FM], unsigned (&)[FM]) const {
+#pragma unroll
+    for (unsigned r = 0; r < ROWS; ++r)
+      load8(x + static_cast<int64_t>(min(r, m - 1)) * stride, static_cast<int>(g * 512 + lane * 8), k, raw.w[r]);
+  }
+  template <int FM>
+  __device__ __forceinline__ void finish(const Raw& raw, unsigned lane, char* lds, u32x4 (&x)[4][FM], unsigned (&sx)[FM]) const {
+    unsigned* codes = reinterpret_cast<unsigned*>(lds);  // [quad][block][row][4 words]
+    unsigned char* scales = reinterpret_cast<unsigned char*>(lds + ROWS * 256);  // [block][row][quad]
+    const unsigned quad = lane >> 4, block = (lane >> 2) & 3;
+    __builtin_amdgcn_wave_barrier();  // the wave's earlier reads are done in order
+#pragma unroll
+    for (unsigned r = 0; r < ROWS; ++r) {
+      unsigned m = 0;
+#pragma unroll
+      for (unsigned v : raw.w[r]) m = Elem<X>::amax(m, v);
+      m = Elem<X>::amax_f32(m);
+      m = max(m, dpp<kXor1>(m));
+      m = max(m, dpp<kXor2>(m));
+      const unsigned byte = scale_byte(m);
+      codes[((lane >> 2) * ROWS + r) * 4 + (lane & 3)] = byte == 255 ? 0u : codes8<X>(raw.w[r], scale_of(byte));
+      if ((lane & 3) == 0) scales[(block * ROWS + r) * 4 + quad] = static_cast<unsigned char>(byte);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    const unsigned r = min(lane & 15, ROWS - 1u), b = lane >> 4;
+#pragma unroll
+    for (unsigned q = 0; q < 4; ++q) x[q][0] = *reinterpret_cast<const u32x4*>(codes + ((q * 4 + b) * ROWS + r) * 4);
+    sx[0] = *reinterpret_cast<const unsigned*>(scales + (b * ROWS + r) * 4);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  }
+};
+
+template <typename T, typename Source, int FM, int R, int U>
+__global__ void __launch_bounds__(64 * kWaves) product_few_rows_kernel(Source source, const char* __restrict__ bc,
+                                                                       const char* __restrict__ bs, unsigned m, unsigned n,
+                                                                       unsigned quads, T* __restrict__ c, int64_t stride) {
+  constexpr int kSums = kWaves * R * FM * 1024;
+  constexpr int kLds = kSums > kWaves * Source::kLds ? kSums : kWaves * Source::kLds;
+  __shared__ __attribute__((aligned(16))) char lds[kLds];
+  const unsigned lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const unsigned rbn = (n + 15) / 16, groups = (quads + 3) / 4, rb0 = blockIdx.x * R;
+  f32x4 acc[R][FM] = {};
+  auto run = [&](auto count, auto full_groups, unsigned g0) {  // `count` groups, kWaves apart
+    constexpr int N = decltype(count)::value;
+    constexpr bool FULL = decltype(full_groups)::value != 0;
+    typename Source::Raw raw[N];
+    u32x4 x[N][4][FM], w[N][R][4];
+    unsigned sx[N][FM], sw[N][R];
+    const unsigned nq = FULL ? 4 : quads - g0 * 4;
+#pragma unroll
+    for (int u = 0; u < N; ++u) source.template load<FM, FULL>(g0 + u * kWaves, nq, lane, raw[u], x[u], sx[u]);
+#pragma unroll
+    for (int u = 0; u < N; ++u)
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const unsigned rb = min(rb0 + r, rbn - 1), g = g0 + u * kWaves;
+        sw[u][r] = *reinterpret_cast<const unsigned*>(bs + (static_cast<size_t>(rb) * groups + g) * 256 + lane * 4);
+#pragma unroll
+        for (unsigned q = 0; q < 4; ++q)
+          if (FULL || q < nq)
+            w[u][r][q] = __builtin_nontemporal_load(
+                reinterpret_cast<const u32x4*>(bc + (static_cast<size_t>(rb) * quads + g * 4 + q) * 1024 + lane * 16));
+          else
+            w[u][r][q] = u32x4{0, 0, 0, 0};
+      }
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      source.template finish<FM>(raw[u], lane, lds + wave * Source::kLds, x[u], sx[u]);
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int f = 0; f < FM; ++f) {
+          acc[r][f] = mfma16<0>(w[u][r][0], x[u][0][f], acc[r][f], sw[u][r], sx[u][f]);
+          acc[r][f] = mfma16<1>(w[u][r][1], x[u][1][f], acc[r][f], sw[u][r], sx[u][f]);
+          acc[r][f] = mfma16<2>(w[u][r][2], x[u][2][f], acc[r][f], sw[u][r], sx[u][f]);
+          acc[r][f] = mfma16<3>(w[u][r][3], x[u][3][f], acc[r][f], sw[u][r], sx[u][f]);
+        }
+    }
+  };
+  const unsigned whole = quads / 4;
+  unsigned g = wave;
+  for (; g + (U - 1) * kWaves < whole; g += U * kWaves) run(Int<U>{}, Int<1>{}, g);
+  for (; g < whole; g += kWaves) run(Int<1>{}, Int<1>{}, g);
+  if (g < groups) run(Int<1>{}, Int<0>{}, g);
+
+  __syncthreads();
+  f32x4* sums = reinterpret_cast<f32x4*>(lds);  // [wave][block][lane]
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int f = 0; f < FM; ++f) sums[((wave * R + r) * FM + f) * 64 + lane] = acc[r][f];
+  __syncthreads();
+  const float* flat = reinterpret_cast<const float*>(lds);
+  // result i of the workgroup: row of x i / (16 R), column i % (16 R), at lane 16 (column % 16 / 4) + row % 16
+  for (unsigned i = threadIdx.x; i < 16u * R * min(m, 16u * FM); i += 64 * kWaves) {
+    const unsigned row = i / (16 * R), col = i % (16 * R);
+    const unsigned at = (((col / 16) * FM + row / 16) * 64 + (col % 16 / 4) * 16 + row % 16) * 4 + col % 4;
+    float v = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) v += flat[w * R * FM * 256 + at];
+    if (rb0 * 16 + col < n) c[static_cast<int64_t>(row) * stride + rb0 * 16 + col] = Elem<T>::from_f32(v);
+  }
+}
+
+template <typename T, int FM, int R, int U, typename Source>
+void launch_few_rows(Source source, const void* bc, const void* bs, int64_t m, int64_t n, int64_t k, T* c,
+                     int64_t stride, hipStream_t s) {
+  hipLaunchKernelGGL((product_few_rows_kernel<T, Source, FM, R, U>), dim3(static_cast<unsigned>((n + 16 * R - 1) / (16 * R))),
+                     dim3(64 * kWaves), 0, s, source, static_cast<const char*>(bc), static_cast<const char*>(bs),
+                     static_cast<unsigned>(m), static_cast<unsigned>(n), static_cast<unsigned>(mx_quads(k)), c, stride);
+}
+
+constexpr int64_t kFusedRows = 16, kFewRows = 64;
+
 void check_product(int64_t m, int64_t n, int64_t k, int64_t stride) {
   require(m >= 0 && n >= 0 && k >= 1, "mx: m and n must be >= 0 and k >= 1");
   require(mx_fits(m, k) && mx_fits(n, k) && ((m + 15) / 16) * ((n + 15) / 16) < (1ll << 28),
@@ -200,7 +361,16 @@ void launch_mx_product(int dev, const void* a_codes, const void* a_scales, const
                          static_cast<unsigned>(m), static_cast<unsigned>(n), static_cast<unsigned>(mx_quads(k)),
                          static_cast<T*>(c), stride, Div(tn));
     };
-    if (m > 1024 && n > 1024) run(product_tile_kernel<T, 8, 8>, 256, 256);
+    if (m <= kFewRows) {
+      const QuantizedRows x{static_cast<const char*>(a_codes), static_cast<const char*>(a_scales),
+                            static_cast<unsigned>(mx_quads(k)), static_cast<unsigned>(mx_groups(k)),
+                            static_cast<unsigned>(mx_row_blocks(m))};
+      auto s = static_cast<hipStream_t>(stream);
+      auto out = static_cast<T*>(c);
+      if (m <= 16) launch_few_rows<T, 1, 1, 2>(x, b_codes, b_scales, m, n, k, out, stride, s);
+      else if (m <= 32) launch_few_rows<T, 2, 2, 2>(x, b_codes, b_scales, m, n, k, out, stride, s);
+      else launch_few_rows<T, 4, 2, 2>(x, b_codes, b_scales, m, n, k, out, stride, s);
+    } else if (m > 1024 && n > 1024) run(product_tile_kernel<T, 8, 8>, 256, 256);
     else if (m > 64 && n > 64) run(product_tile_kernel<T, 4, 4>, 128, 128);
     else run(product_tile_kernel<T, 2, 2>, 64, 64);
   });
@@ -208,13 +378,39 @@ void launch_mx_product(int dev, const void* a_codes, const void* a_scales, const
 }
 
 size_t mx_linear_workspace(int dev, int64_t m, int64_t n, int64_t k) {
+  check_product(m, n, k, n);
+  if (m <= kFusedRows) return 0;
   return round16(static_cast<size_t>(mx_codes_bytes(m, k) + mx_scales_bytes(m, k))) + mx_product_workspace(dev, m, n, k);
 }
 
 void launch_mx_linear(int dev, const void* x, const std::string& dtype, int64_t x_stride, const void* w_codes,
                       const void* w_scales, int64_t m, int64_t n, int64_t k, void* y, int64_t y_stride,
                       void* workspace, size_t workspace_bytes, void* stream) {
-  require(workspace_bytes >= mx_linear_workspace(dev, m, n, k), "mx_linear: workspace too small");
+  const Type t = type_of(dtype, "mx_linear: dtype must be bf16|f16|f32");
+  check_product(m, n, k, y_stride);
+  require(x_stride >= k || m <= 1, "mx_linear: x_stride must be at least k");
+  if (m == 0 || n == 0) return;
+  require(x && w_codes && w_scales && y, "mx_linear: null pointer");
+  require(aligned(x, size_of(t)) && aligned(y, size_of(t)) && aligned(w_codes, 16) && aligned(w_scales, 16),
+          "mx_linear: x and y aligned to their type, codes and scales to 16 bytes");
+  if (m <= kFusedRows) {
+    OnDevice on(dev);
+    auto s = static_cast<hipStream_t>(stream);
+    with_type(t, [&](auto e) {
+      using T = decltype(e);
+      auto px = static_cast<const T*>(x);
+      auto out = static_cast<T*>(y);
+      const auto rows = static_cast<unsigned>(m);
+      const int len = static_cast<int>(k);
+      if (m == 1) launch_few_rows<T, 1, 1, 2>(PlainRows<T, 1>{px, x_stride, rows, len}, w_codes, w_scales, m, n, k, out, y_stride, s);
+      else if (m <= 4) launch_few_rows<T, 1, 1, 2>(PlainRows<T, 4>{px, x_stride, rows, len}, w_codes, w_scales, m, n, k, out, y_stride, s);
+      else if (m <= 8) launch_few_rows<T, 1, 2, 1>(PlainRows<T, 8>{px, x_stride, rows, len}, w_codes, w_scales, m, n, k, out, y_stride, s);
+      else launch_few_rows<T, 1, 2, 1>(PlainRows<T, 16>{px, x_stride, rows, len}, w_codes, w_scales, m, n, k, out, y_stride, s);
+    });
+    check(hipGetLastError(), "mx_linear");
+    return;
+  }
+  require(workspace && workspace_bytes >= mx_linear_workspace(dev, m, n, k), "mx_linear: workspace too small");
   require(aligned(workspace, 16), "mx_linear: workspace aligned to 16 bytes");
   auto codes = static_cast<char*>(workspace);
   auto scales = codes + mx_codes_bytes(m, k);
