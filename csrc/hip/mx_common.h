@@ -126,7 +126,9 @@ struct Div {
     m = static_cast<unsigned>((1ull << (31 + l)) / div + 1);
     s = l - 1;
   }
-  __device__ __forceinline__ unsigned quot(unsigned x) const { return d == 1 ? x : __umulhi(x, m) >> s; }
+  __device__ __forceinline__ unsigned quot(unsigned x) const {
+    return d == 1 ? x : static_cast<unsigned>((static_cast<uint64_t>(x) * m) >> 32) >> s;
+  }
 };
 
 // ---- host ------------------------------------------------------------------------------------

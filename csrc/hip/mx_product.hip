@@ -1,4 +1,7 @@
 // MXFP4 product and linear layer (format and layout: mx.h).
+#include <algorithm>
+#include <atomic>
+
 #include "mx_common.h"
 
 namespace gpumon_hip {
@@ -6,7 +9,6 @@ namespace mx {
 namespace {
 
 typedef __attribute__((address_space(3))) void LdsVoid;
-typedef const __attribute__((address_space(1))) void GlobalVoid;
 
 // One wave's 16x16x128 step on one chunk of either side; S picks the quad's byte of the scale words.
 // D: lane l holds row l & 15 of b's chunk and rows 4 (l >> 4) + i of a's.
@@ -20,144 +22,268 @@ __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c, unsigned sa, 
 // s_waitcnt with a vmcnt and, if lgkm0, lgkmcnt(0).
 constexpr int wait_imm(int vm, bool lgkm0) { return (vm & 15) | ((vm >> 4) << 14) | (7 << 4) | ((lgkm0 ? 0 : 15) << 8); }
 
+// Buffers: a uniform base, offsets of 32 bits of which one is uniform; past `size` reads give zeros.
+typedef __amdgpu_buffer_rsrc_t Buffer;
+__device__ __forceinline__ Buffer buffer(const char* base, unsigned size) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, static_cast<int>(size), 0x00020000);
+}
+// 16 bytes a lane to LDS, lane after lane.
+__device__ __forceinline__ void load_lds(Buffer b, unsigned offset, unsigned uniform, char* lds) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(b, (LdsVoid*)lds, 16, static_cast<int>(offset), static_cast<int>(uniform), 0, 0);
+}
+
 template <int S>
 using Int = std::integral_constant<int, S>;
 
-// 2 x 2 waves, FM x FN chunks of 16 x 16 results each.
-template <typename T, int FM, int FN>
-__global__ void __launch_bounds__(256, FM* FN > 32 ? 1 : 2)
+// The tiles of a product in the order in which the workgroups take them: bands of eight rows of tiles,
+// down each column of a band. Workgroups run on the eight XCDs in turn, and each XCD takes a run of
+// neighbours in this order (with 32 CUs, 8 x 4 tiles), so that its cache sees each operand's rows once.
+struct Tiles {
+  unsigned rows, cols, total;
+  Div band, last;  // tiles of a band; rows of the last band
+  Tiles(unsigned r, unsigned c) : rows(r), cols(c), total(r * c), band(8 * c), last((r + 7) % 8 + 1) {}
+  // tile `r` of this workgroup; false if it has none
+  __device__ __forceinline__ bool get(unsigned r, unsigned& row, unsigned& col) const {
+    const unsigned first = r * gridDim.x, place = blockIdx.x / 8;
+    const unsigned count = first < total ? min(total - first, gridDim.x) : 0, per = (count + 7) / 8;
+    const unsigned p = blockIdx.x % 8 * per + place, b = band.quot(first + p), in = first + p - b * band.d;
+    const bool whole = b * 8 + 8 <= rows;
+    col = whole ? in / 8 : last.quot(in);
+    row = b * 8 + in - col * (whole ? 8 : last.d);
+    row = __builtin_amdgcn_readfirstlane(row), col = __builtin_amdgcn_readfirstlane(col);
+    return place < per && p < count;
+  }
+};
+
+// The order of a stage's work in a wave: FM x FN matrix instructions, row after row, and between them,
+// evenly, the next stages' loads (kLoad), and the next stage's operands from LDS: b's (kB), a's last TAIL
+// rows (kTail), for both of which there are two sets of registers, and a's other rows (kA), each into the
+// registers of its row once that row is done.
+enum Op { kLoad, kB, kTail, kA };
+template <int FM, int FN, int LOADS>
+struct Order {
+  static constexpr int kTails = FM / 4 > 0 ? FM / 4 : 1, kOps = LOADS + FN + FM;
+  Op op[kOps] = {};
+  int index[kOps] = {}, before[kOps] = {};  // matrix instructions before it
+  constexpr Order() {
+    int load = 0, b = 0, tail = 0, a = 0;
+    for (int o = 0; o < kOps; ++o) {
+      before[o] = (o + 1) * FM * FN / (kOps + 1);
+      if (a < FM - kTails && before[o] >= (a + 1) * FN) op[o] = kA, index[o] = a++;
+      else if (tail < kTails) op[o] = kTail, index[o] = tail++;
+      else if (load < LOADS && load <= b) op[o] = kLoad, index[o] = load++;
+      else if (b < FN) op[o] = kB, index[o] = b++;
+      else if (load < LOADS) op[o] = kLoad, index[o] = load++;
+      else op[o] = kA, before[o] = (a + 1) * FN, index[o] = a++;
+    }
+  }
+};
+
+template <int O, int FM, int FN, int LOADS>
+__device__ __forceinline__ void hold() {
+  constexpr Order<FM, FN, LOADS> order;
+  if constexpr (O < order.kOps) {
+    constexpr int before = order.before[O] - (O ? order.before[O ? O - 1 : 0] : 0);
+    if constexpr (before > 0) __builtin_amdgcn_sched_group_barrier(0x008, before, 0);
+    __builtin_amdgcn_sched_group_barrier(order.op[O] == kLoad ? 0x010 : 0x100, 1, 0);
+    hold<O + 1, FM, FN, LOADS>();
+  } else {
+    __builtin_amdgcn_sched_group_barrier(0x008, FM * FN - order.before[order.kOps - 1], 0);
+  }
+}
+
+// WM x WN waves, FM x FN chunks of 16 x 16 results each. The stages (a quad of every chunk of the tile)
+// go through LDS in four slots, loaded three stages ahead, without a break from one tile to the next;
+// a stage's operands are read into registers while the one before multiplies, so that the matrix
+// instructions wait for nothing but the barrier (Order). b's rows take the instruction's A side: a lane's four
+// sums are neighbours in a row of c.
+template <typename T, int FM, int FN, int WM, int WN, int RESIDENT>
+__global__ void __launch_bounds__(64 * WM * WN, RESIDENT * WM * WN / 4)
     product_tile_kernel(const char* __restrict__ ac, const char* __restrict__ as, const char* __restrict__ bc,
                         const char* __restrict__ bs, unsigned m, unsigned n, unsigned quads, T* __restrict__ c,
-                        int64_t stride, Div tiles_n) {
-  constexpr int kChunks = 2 * (FM + FN), kLoads = kChunks / 4, kScaleLoads = kChunks >= 16 ? kChunks / 16 : 1;
+                        int64_t stride, Tiles tiles) {
+  constexpr int TM = FM * WM, TN = FN * WN, kChunks = TM + TN, kLoads = kChunks / (WM * WN);
+  constexpr int kScaleLoads = kChunks >= 4 * WM * WN ? kChunks / (4 * WM * WN) : 1;
   constexpr int kStage = kChunks * 1024, kScales = kChunks * 256;
-  __shared__ __attribute__((aligned(16))) char lds[4 * kStage + 2 * kScales];
+  // results leave through LDS in pieces of 16 rows x up to 128 bytes, kParts times 16 bytes a row
+  constexpr int kPiece = 8 / static_cast<int>(sizeof(T)) < FN ? 8 / static_cast<int>(sizeof(T)) : FN;
+  constexpr int kParts = kPiece * static_cast<int>(sizeof(T)), kOut = 256 * kParts;
+  __shared__ __attribute__((aligned(16))) char lds[4 * kStage + 2 * kScales + WM * WN * kOut];
   const unsigned lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const unsigned tm = tiles_n.quot(blockIdx.x), tn = blockIdx.x - tm * tiles_n.d;
   const unsigned rbm = (m + 15) / 16, rbn = (n + 15) / 16, groups = (quads + 3) / 4;
-  const unsigned wm = wave & 1, wn = wave >> 1;
+  const unsigned wm = wave % WM, wn = wave / WM;
 
-  // chunk `x` of the tile, a's 2 FM first; row blocks past the end read the last one instead, and what
-  // comes of them is not stored
-  auto row_block = [&](unsigned x) {
-    return x < 2 * FM ? min(tm * (2 * FM) + x, rbm - 1) : min(tn * (2 * FN) + x - 2 * FM, rbn - 1);
+  Buffer src[kLoads], ssrc[kScaleLoads];
+  unsigned soff[kScaleLoads];  // four chunks' scales a load, 16 lanes each; TM is a multiple of 4
+  // Where the loads come from: chunk x of a tile, a's TM first. Row blocks past the end read the last one
+  // instead, and what comes of them is not stored. Past the last tile, and past the last quad, zeros come
+  // without a read: four steps at a time are taken, and scales there are zeros too.
+  auto aim = [&](bool any, unsigned tm, unsigned tn) {
+    auto row_block = [&](unsigned x) {
+      return x < TM ? min(tm * TM + x, rbm - 1) : min(tn * TN + x - TM, rbn - 1);
+    };
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const unsigned x = wave * kLoads + i;
+      src[i] = buffer((x < TM ? ac : bc) + static_cast<size_t>(row_block(x)) * quads * 1024, any ? quads * 1024 : 0);
+    }
+#pragma unroll
+    for (int i = 0; i < kScaleLoads; ++i) {
+      const unsigned x = (wave * kScaleLoads + i) * 4 % kChunks, first = row_block(x);
+      ssrc[i] = buffer((x < TM ? as : bs) + static_cast<size_t>(first) * groups * 256,
+                       any ? (row_block(x + 3) - first + 1) * groups * 256 : 0);
+      soff[i] = (row_block(x + (lane >> 4)) - first) * groups * 256 + (lane & 15) * 16;
+    }
   };
-  const char* src[kLoads];
-#pragma unroll
-  for (int i = 0; i < kLoads; ++i) {
-    const unsigned x = wave * kLoads + i;
-    src[i] = (x < 2 * FM ? ac : bc) + static_cast<size_t>(row_block(x)) * quads * 1024;
-  }
-  const char* ssrc[kScaleLoads];
-#pragma unroll
-  for (int i = 0; i < kScaleLoads; ++i) {
-    const unsigned x = ((wave * kScaleLoads + i) * 4 + (lane >> 4)) % kChunks;
-    ssrc[i] = (x < 2 * FM ? as : bs) + static_cast<size_t>(row_block(x)) * groups * 256 + (lane & 15) * 16;
-  }
-  auto load_stage = [&](unsigned t, int slot) {
-    const unsigned q = min(t, quads - 1);
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i)
-      __builtin_amdgcn_global_load_lds((GlobalVoid*)(src[i] + static_cast<size_t>(q) * 1024 + lane * 16),
-                                       (LdsVoid*)(lds + slot * kStage + (wave * kLoads + i) * 1024), 16, 0, 0);
+  auto load_chunk = [&](int i, unsigned at, int slot) {
+    load_lds(src[i], lane * 16, at, lds + slot * kStage + (wave * kLoads + i) * 1024);
   };
-  auto load_scales = [&](unsigned g) {
-    const unsigned q = min(g, groups - 1);
+  auto load_scales = [&](unsigned g, unsigned half) {
 #pragma unroll
     for (int i = 0; i < kScaleLoads; ++i)
-      __builtin_amdgcn_global_load_lds(
-          (GlobalVoid*)(ssrc[i] + static_cast<size_t>(q) * 256),
-          (LdsVoid*)(lds + 4 * kStage + (g & 1) * kScales + (wave * kScaleLoads + i) * 1024 % kScales), 16, 0, 0);
+      load_lds(ssrc[i], soff[i], g * 256, lds + 4 * kStage + half * kScales + (wave * kScaleLoads + i) * 1024 % kScales);
   };
 
-  u32x4 fa[2][FM], fb[2][FN];
-  unsigned sa[FM], sb[FN], sa2[FM], sb2[FN];
-  f32x4 acc[FM][FN] = {};
-  auto read_stage = [&](int slot, u32x4* a, u32x4* b) {
-    const char* p = lds + slot * kStage + lane * 16;
-#pragma unroll
-    for (int i = 0; i < FM; ++i) a[i] = *reinterpret_cast<const u32x4*>(p + (wm * FM + i) * 1024);
-#pragma unroll
-    for (int j = 0; j < FN; ++j) b[j] = *reinterpret_cast<const u32x4*>(p + (2 * FM + wn * FN + j) * 1024);
+  constexpr Order<FM, FN, kLoads> order;
+  constexpr int kTails = order.kTails, kHead = FM - kTails;
+  u32x4 fa[kHead], ft[2][kTails], fb[2][FN];
+  unsigned sa[FM], sb[FN];
+  f32x4 acc[FM][FN];
+  auto read_a = [&](int x, int slot) {
+    return *reinterpret_cast<const u32x4*>(lds + slot * kStage + lane * 16 + (wm * FM + x) * 1024);
   };
-  auto read_scales = [&](unsigned g, unsigned* a, unsigned* b) {
-    const char* p = lds + 4 * kStage + (g & 1) * kScales + lane * 4;
+  auto read_b = [&](int x, int slot) {
+    return *reinterpret_cast<const u32x4*>(lds + slot * kStage + lane * 16 + (TM + wn * FN + x) * 1024);
+  };
+  auto read_scales = [&](unsigned half) {
+    const char* p = lds + 4 * kStage + half * kScales + lane * 4;
 #pragma unroll
-    for (int i = 0; i < FM; ++i) a[i] = *reinterpret_cast<const unsigned*>(p + (wm * FM + i) * 256);
+    for (int i = 0; i < FM; ++i) sa[i] = *reinterpret_cast<const unsigned*>(p + (wm * FM + i) * 256);
 #pragma unroll
-    for (int j = 0; j < FN; ++j) b[j] = *reinterpret_cast<const unsigned*>(p + (2 * FM + wn * FN + j) * 256);
+    for (int j = 0; j < FN; ++j) sb[j] = *reinterpret_cast<const unsigned*>(p + (TM + wn * FN + j) * 256);
   };
 
-  load_scales(0);
+  unsigned tm = 0, tn = 0, round = 0;
+  if (!tiles.get(0, tm, tn)) return;
+  aim(true, tm, tn);
+  load_scales(0, 0);
 #pragma unroll
-  for (int t = 0; t < 4; ++t) load_stage(t, t);
+  for (int t = 0; t < 4; ++t)
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) load_chunk(i, t * 1024, t);
   __builtin_amdgcn_s_waitcnt(wait_imm(3 * kLoads, false));
   __builtin_amdgcn_s_barrier();
-  read_scales(0, sa, sb);
-  read_stage(0, fa[0], fb[0]);
+  read_scales(0);
+#pragma unroll
+  for (int x = 0; x < kHead; ++x) fa[x] = read_a(x, 0);
+#pragma unroll
+  for (int x = 0; x < kTails; ++x) ft[0][x] = read_a(kHead + x, 0);
+#pragma unroll
+  for (int x = 0; x < FN; ++x) fb[0][x] = read_b(x, 0);
 
+  unsigned half = 0;     // of the scales' two places, the one in use
   auto body = [&](unsigned g, auto step) {
     constexpr int J = decltype(step)::value;
-    const unsigned t = g * 4 + J;
-    // stage t + 1 is here, for every wave, and every wave has read stage t
-    __builtin_amdgcn_s_waitcnt(wait_imm(2 * kLoads + (J == 1 || J == 2 ? kScaleLoads : 0), true));
+    // stage g * 4 + J + 1 is here, for every wave, and every wave has read the one before it
+    constexpr int kAfter = 2 * kLoads + (J == 1 || J == 2 ? kScaleLoads : 0);
+    __builtin_amdgcn_s_waitcnt(wait_imm(kAfter, true));
     __builtin_amdgcn_s_barrier();
     __builtin_amdgcn_sched_barrier(0);
-    if constexpr (J == 0) load_scales(g + 1);
-    load_stage(t + 4, J);
-    read_stage((J + 1) & 3, fa[(J + 1) & 1], fb[(J + 1) & 1]);
-    if constexpr (J == 3) read_scales(g + 1, sa2, sb2);
+    constexpr int kNow = J & 1, kNext = kNow ^ 1, kSlot = (J + 1) & 3;
+    const bool last = g + 1 == groups;  // then the next tile's loads
+    const unsigned at = last ? J * 1024 : (g * 4 + J + 4) * 1024;
+    auto multiply = [&](int from, int to) {
+#pragma unroll
+      for (int x = from; x < to; ++x) {
+        const int i = x / FN, j = x % FN;
+        acc[i][j] = mfma16<J>(fb[kNow][j], i < kHead ? fa[i] : ft[kNow][i - kHead], acc[i][j], sb[j], sa[i]);
+      }
+    };
+    if constexpr (J == 0) load_scales(last ? 0 : g + 1, half ^ 1);
+#pragma unroll
+    for (int o = 0; o < order.kOps; ++o) {
+      multiply(o ? order.before[o - 1] : 0, order.before[o]);
+      const int x = order.index[o];
+      if (order.op[o] == kLoad) load_chunk(x, at, J);
+      else if (order.op[o] == kB) fb[kNext][x] = read_b(x, kSlot);
+      else if (order.op[o] == kTail) ft[kNext][x] = read_a(kHead + x, kSlot);
+      else fa[x] = read_a(x, kSlot);
+    }
+    multiply(order.before[order.kOps - 1], FM * FN);
+    // and the scheduler is held to it
+    if constexpr (J == 0) __builtin_amdgcn_sched_group_barrier(0x010, kScaleLoads, 0);
+    hold<0, FM, FN, kLoads>();
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (J == 3) {
+      half ^= 1;
+      read_scales(half);
+    }
+  };
+
+  for (;;) {
 #pragma unroll
     for (int i = 0; i < FM; ++i)
 #pragma unroll
-      for (int j = 0; j < FN; ++j)
-        acc[i][j] = mfma16<J>(fb[J & 1][j], fa[J & 1][i], acc[i][j], sb[j], sa[i]);
-    if constexpr (J == 3) {
-#pragma unroll
-      for (int i = 0; i < FM; ++i) sa[i] = sa2[i];
-#pragma unroll
-      for (int j = 0; j < FN; ++j) sb[j] = sb2[j];
+      for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+    unsigned next_m = 0, next_n = 0;
+    const bool more = tiles.get(round + 1, next_m, next_n);
+#pragma unroll 1
+    for (unsigned g = 0; g < groups; ++g) {
+      if (g + 1 == groups) aim(more, next_m, next_n);
+      body(g, Int<0>{});
+      body(g, Int<1>{});
+      body(g, Int<2>{});
+      body(g, Int<3>{});
     }
-#pragma unroll
-    for (int i = 0; i < FM + FN; ++i) {  // one read of LDS, then its share of the matrix instructions
-      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x008, FM * FN / (FM + FN), 0);
-    }
-    __builtin_amdgcn_sched_barrier(0);
-  };
-  const unsigned whole = quads / 4, rest = quads & 3;
-  for (unsigned g = 0; g < whole; ++g) {
-    body(g, Int<0>{});
-    body(g, Int<1>{});
-    body(g, Int<2>{});
-    body(g, Int<3>{});
-  }
-  if (rest > 0) body(whole, Int<0>{});
-  if (rest > 1) body(whole, Int<1>{});
-  if (rest > 2) body(whole, Int<2>{});
-  __builtin_amdgcn_s_waitcnt(wait_imm(0, true));  // nothing may arrive after the workgroup's memory is given back
 
-  const unsigned row0 = (tm * 2 + wm) * FM * 16 + (lane & 15), col0 = (tn * 2 + wn) * FN * 16 + (lane >> 4) * 4;
+    unsigned l = lane;
+    asm volatile("" : "+v"(l));  // what follows from the lane is computed here, not kept through the loop above
+    const unsigned row0 = (tm * WM + wm) * FM * 16, col0 = (tn * WN + wn) * FN * 16, r = l & 15, q = l >> 4;
+    T* out = c + static_cast<int64_t>(row0) * stride + col0;
+    char* piece = lds + 4 * kStage + 2 * kScales + wave * kOut;
+    auto leave = [&](auto store) {
 #pragma unroll
-  for (int i = 0; i < FM; ++i) {
-    const unsigned row = row0 + i * 16;
-    if (row >= m) continue;
-    T* out = c + static_cast<int64_t>(row) * stride;
+      for (int i = 0; i < FM; ++i)
 #pragma unroll
-    for (int j = 0; j < FN; ++j) {
-      const unsigned col = col0 + j * 16;
-      T v[4];
+        for (int h = 0; h < FN; h += kPiece) {
+          // the 16-byte parts' places in a row are mixed by the row: neither writes nor reads meet in a bank
+          __builtin_amdgcn_wave_barrier();
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = Elem<T>::from_f32(acc[i][j][e]);
-      if (col + 4 <= n) {
-        __builtin_memcpy(out + col, v, sizeof(v));
-      } else {
+          for (unsigned j = 0; j < kPiece; ++j) {
+            T v[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (col + e < n) out[col + e] = v[e];
-      }
+            for (int e = 0; e < 4; ++e) v[e] = Elem<T>::from_f32(acc[i][h + j][e]);
+            const unsigned at = (j * 4 + q) * sizeof(v);  // in the row
+            __builtin_memcpy(__builtin_assume_aligned(piece + r * (16 * kParts) + ((at / 16) ^ (r % kParts)) * 16 + at % 16, sizeof(v)), v, sizeof(v));
+          }
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+          __builtin_amdgcn_wave_barrier();
+#pragma unroll
+          for (unsigned o = 0; o < kParts / 4; ++o) {
+            const unsigned row = o * (64 / kParts) + l / kParts, part = l % kParts;
+            T v[16 / sizeof(T)];
+            __builtin_memcpy(v, __builtin_assume_aligned(piece + row * (16 * kParts) + (part ^ (row % kParts)) * 16, 16), 16);
+            store(i * 16 + row, h * 16 + part * (16 / sizeof(T)), v);
+          }
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        }
+    };
+    if (__builtin_amdgcn_readfirstlane(row0 + FM * 16 <= m && col0 + FN * 16 <= n)) {
+      leave([&](unsigned row, unsigned col, const T* v) {
+        __builtin_memcpy(out + static_cast<int64_t>(row) * stride + col, v, 16);
+      });
+    } else {
+      leave([&](unsigned row, unsigned col, const T* v) {
+        if (row0 + row >= m) return;
+#pragma unroll
+        for (unsigned e = 0; e < 16 / sizeof(T); ++e)
+          if (col0 + col + e < n) out[static_cast<int64_t>(row) * stride + col + e] = v[e];
+      });
     }
+    if (!more) break;
+    tm = next_m, tn = next_n, ++round;
   }
+  __builtin_amdgcn_s_waitcnt(wait_imm(0, true));  // no load may arrive after the workgroup's memory is given back
 }
 
 // ---- few rows ----------------------------------------------------------------------------------
@@ -319,6 +445,18 @@ void launch_few_rows(Source source, const void* bc, const void* bs, int64_t m, i
                      static_cast<unsigned>(m), static_cast<unsigned>(n), static_cast<unsigned>(mx_quads(k)), c, stride);
 }
 
+// Compute units, asked for once a device (a multiple of eight: whole XCDs).
+int compute_units(int dev) {
+  static std::atomic<int> known[64];
+  if (dev < 0 || dev >= 64) return device_cu_count(dev);
+  int n = known[dev].load(std::memory_order_relaxed);
+  if (n == 0) {
+    n = std::max(8, device_cu_count(dev) / 8 * 8);
+    known[dev].store(n, std::memory_order_relaxed);
+  }
+  return n;
+}
+
 constexpr int64_t kFusedRows = 16, kFewRows = 64;
 
 void check_product(int64_t m, int64_t n, int64_t k, int64_t stride) {
@@ -353,13 +491,14 @@ void launch_mx_product(int dev, const void* a_codes, const void* a_scales, const
   OnDevice on(dev);
   with_type(t, [&](auto e) {
     using T = decltype(e);
-    auto run = [&](auto kernel, int tile_m, int tile_n) {
+    auto run = [&](auto kernel, int tile_m, int tile_n, int waves, int resident) {
       const unsigned tn = static_cast<unsigned>((n + tile_n - 1) / tile_n), tm = static_cast<unsigned>((m + tile_m - 1) / tile_m);
-      hipLaunchKernelGGL(kernel, dim3(tm * tn), dim3(256), 0, static_cast<hipStream_t>(stream),
+      const unsigned total = tm * tn, grid = std::min((total + 7) / 8 * 8, static_cast<unsigned>(compute_units(dev) * resident));
+      hipLaunchKernelGGL(kernel, dim3(grid), dim3(64 * waves), 0, static_cast<hipStream_t>(stream),
                          static_cast<const char*>(a_codes), static_cast<const char*>(a_scales),
                          static_cast<const char*>(b_codes), static_cast<const char*>(b_scales),
                          static_cast<unsigned>(m), static_cast<unsigned>(n), static_cast<unsigned>(mx_quads(k)),
-                         static_cast<T*>(c), stride, Div(tn));
+                         static_cast<T*>(c), stride, Tiles(tm, tn));
     };
     if (m <= kFewRows) {
       const QuantizedRows x{static_cast<const char*>(a_codes), static_cast<const char*>(a_scales),
@@ -370,9 +509,15 @@ void launch_mx_product(int dev, const void* a_codes, const void* a_scales, const
       if (m <= 16) launch_few_rows<T, 1, 1, 2>(x, b_codes, b_scales, m, n, k, out, stride, s);
       else if (m <= 32) launch_few_rows<T, 2, 2, 2>(x, b_codes, b_scales, m, n, k, out, stride, s);
       else launch_few_rows<T, 4, 2, 2>(x, b_codes, b_scales, m, n, k, out, stride, s);
-    } else if (m > 1024 && n > 1024) run(product_tile_kernel<T, 8, 8>, 256, 256);
-    else if (m > 64 && n > 64) run(product_tile_kernel<T, 4, 4>, 128, 128);
-    else run(product_tile_kernel<T, 2, 2>, 64, 64);
+    } else if (m > 1024 && n > 1024) { const char* v = getenv("MXV"); int w = v ? atoi(v) : 0;
+      if (w == 0) run(product_tile_kernel<T, 8, 4, 2, 4, 1>, 256, 256, 8, 1);
+      else if (w == 1) run(product_tile_kernel<T, 8, 8, 2, 2, 1>, 256, 256, 4, 1);
+      else if (w == 2) run(product_tile_kernel<T, 4, 8, 4, 2, 1>, 256, 256, 8, 1);
+      else if (w == 3) run(product_tile_kernel<T, 4, 4, 2, 2, 2>, 128, 128, 4, 2);
+      else if (w == 4) run(product_tile_kernel<T, 8, 4, 2, 2, 1>, 256, 128, 4, 1);
+      else run(product_tile_kernel<T, 4, 4, 4, 2, 1>, 256, 128, 8, 1); }
+    else if (m > 64 && n > 64) run(product_tile_kernel<T, 4, 4, 2, 2, 2>, 128, 128, 4, 2);
+    else run(product_tile_kernel<T, 2, 2, 2, 2, 2>, 64, 64, 4, 2);
   });
   check(hipGetLastError(), "mx_product");
 }
