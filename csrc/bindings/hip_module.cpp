@@ -62,7 +62,7 @@ PYBIND11_MODULE(_hip, m) {
     launch_mx_dequantize(dev, P(codes), P(scales), rows, k, P(out), dtype, stride, P(stream));
   }, py::arg("dev"), py::arg("codes"), py::arg("scales"), py::arg("rows"), py::arg("k"), py::arg("out"),
      py::arg("dtype"), py::arg("stride"), py::arg("stream") = 0);
-  m.def("mx_product_workspace", &mx_product_workspace, py::arg("dev"), py::arg("m"), py::arg("n"), py::arg("k"));
+  m.def("mx_product_workspace", &mx_product_workspace, py::arg("m"), py::arg("n"), py::arg("k"));
   m.def("mx_product", [](int dev, uintptr_t a_codes, uintptr_t a_scales, uintptr_t b_codes, uintptr_t b_scales,
                          int64_t m, int64_t n, int64_t k, uintptr_t c, const std::string& dtype, int64_t stride,
                          uintptr_t workspace, size_t workspace_bytes, uintptr_t stream) {
@@ -71,7 +71,7 @@ PYBIND11_MODULE(_hip, m) {
   }, py::arg("dev"), py::arg("a_codes"), py::arg("a_scales"), py::arg("b_codes"), py::arg("b_scales"), py::arg("m"),
      py::arg("n"), py::arg("k"), py::arg("c"), py::arg("dtype"), py::arg("stride"), py::arg("workspace") = 0,
      py::arg("workspace_bytes") = 0, py::arg("stream") = 0);
-  m.def("mx_linear_workspace", &mx_linear_workspace, py::arg("dev"), py::arg("m"), py::arg("n"), py::arg("k"));
+  m.def("mx_linear_workspace", &mx_linear_workspace, py::arg("m"), py::arg("n"), py::arg("k"));
   m.def("mx_linear", [](int dev, uintptr_t x, const std::string& dtype, int64_t x_stride, uintptr_t w_codes,
                         uintptr_t w_scales, int64_t m, int64_t n, int64_t k, uintptr_t y, int64_t y_stride,
                         uintptr_t workspace, size_t workspace_bytes, uintptr_t stream) {

@@ -51,12 +51,12 @@ void launch_mx_quantize_both(int dev, const void* x, const std::string& dtype, i
 void launch_mx_dequantize(int dev, const void* codes, const void* scales, int64_t rows, int64_t k, void* out,
                           const std::string& dtype, int64_t stride, void* stream);
 // c [m, n] = a [m, k] b [n, k]^T, sums in 32 bits, rounded once. workspace: mx_product_workspace bytes.
-size_t mx_product_workspace(int dev, int64_t m, int64_t n, int64_t k);
+size_t mx_product_workspace(int64_t m, int64_t n, int64_t k);
 void launch_mx_product(int dev, const void* a_codes, const void* a_scales, const void* b_codes, const void* b_scales,
                        int64_t m, int64_t n, int64_t k, void* c, const std::string& dtype, int64_t stride,
                        void* workspace, size_t workspace_bytes, void* stream);
 // y [m, n] = Q(x) w^T: x [m, k] in `dtype`, quantised here; y has the same type.
-size_t mx_linear_workspace(int dev, int64_t m, int64_t n, int64_t k);
+size_t mx_linear_workspace(int64_t m, int64_t n, int64_t k);
 void launch_mx_linear(int dev, const void* x, const std::string& dtype, int64_t x_stride, const void* w_codes,
                       const void* w_scales, int64_t m, int64_t n, int64_t k, void* y, int64_t y_stride,
                       void* workspace, size_t workspace_bytes, void* stream);

@@ -97,11 +97,13 @@ __device__ __forceinline__ void hold() {
 // a stage's operands are read into registers while the one before multiplies, so that the matrix
 // instructions wait for nothing but the barrier (Order). b's rows take the instruction's A side: a lane's four
 // sums are neighbours in a row of c.
-template <typename T, int FM, int FN, int WM, int WN, int RESIDENT>
+// SPLIT: the tiles' columns are taken `parts` times, each time with `per` of k's groups of quads, and each
+// part's sums go to a matrix of its own.
+template <typename T, int FM, int FN, int WM, int WN, int RESIDENT, bool SPLIT = false>
 __global__ void __launch_bounds__(64 * WM * WN, RESIDENT * WM * WN / 4)
     product_tile_kernel(const char* __restrict__ ac, const char* __restrict__ as, const char* __restrict__ bc,
                         const char* __restrict__ bs, unsigned m, unsigned n, unsigned quads, T* __restrict__ c,
-                        int64_t stride, Tiles tiles) {
+                        int64_t stride, Tiles tiles, Div part_cols, unsigned per) {
   constexpr int TM = FM * WM, TN = FN * WN, kChunks = TM + TN, kLoads = kChunks / (WM * WN);
   constexpr int kScaleLoads = kChunks >= 4 * WM * WN ? kChunks / (4 * WM * WN) : 1;
   constexpr int kStage = kChunks * 1024, kScales = kChunks * 256;
@@ -110,7 +112,7 @@ __global__ void __launch_bounds__(64 * WM * WN, RESIDENT * WM * WN / 4)
   constexpr int kParts = kPiece * static_cast<int>(sizeof(T)), kOut = 256 * kParts;
   __shared__ __attribute__((aligned(16))) char lds[4 * kStage + 2 * kScales + WM * WN * kOut];
   const unsigned lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const unsigned rbm = (m + 15) / 16, rbn = (n + 15) / 16, groups = (quads + 3) / 4;
+  const unsigned rbm = (m + 15) / 16, rbn = (n + 15) / 16, all_groups = (quads + 3) / 4;
   const unsigned wm = wave % WM, wn = wave / WM;
 
   Buffer src[kLoads], ssrc[kScaleLoads];
@@ -119,20 +121,27 @@ __global__ void __launch_bounds__(64 * WM * WN, RESIDENT * WM * WN / 4)
   // instead, and what comes of them is not stored. Past the last tile, and past the last quad, zeros come
   // without a read: four steps at a time are taken, and scales there are zeros too.
   auto aim = [&](bool any, unsigned tm, unsigned tn) {
+    unsigned g0 = 0;
+    if constexpr (SPLIT) {
+      const unsigned part = part_cols.quot(tn);
+      tn -= part * part_cols.d;
+      g0 = part * per;
+    }
     auto row_block = [&](unsigned x) {
       return x < TM ? min(tm * TM + x, rbm - 1) : min(tn * TN + x - TM, rbn - 1);
     };
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       const unsigned x = wave * kLoads + i;
-      src[i] = buffer((x < TM ? ac : bc) + static_cast<size_t>(row_block(x)) * quads * 1024, any ? quads * 1024 : 0);
+      src[i] = buffer((x < TM ? ac : bc) + (static_cast<size_t>(row_block(x)) * quads + g0 * 4) * 1024,
+                      any ? (quads - g0 * 4) * 1024 : 0);
     }
 #pragma unroll
     for (int i = 0; i < kScaleLoads; ++i) {
       const unsigned x = (wave * kScaleLoads + i) * 4 % kChunks, first = row_block(x);
-      ssrc[i] = buffer((x < TM ? as : bs) + static_cast<size_t>(first) * groups * 256,
-                       any ? (row_block(x + 3) - first + 1) * groups * 256 : 0);
-      soff[i] = (row_block(x + (lane >> 4)) - first) * groups * 256 + (lane & 15) * 16;
+      ssrc[i] = buffer((x < TM ? as : bs) + (static_cast<size_t>(first) * all_groups + g0) * 256,
+                       any ? ((row_block(x + 3) - first + 1) * all_groups - g0) * 256 : 0);
+      soff[i] = (row_block(x + (lane >> 4)) - first) * all_groups * 256 + (lane & 15) * 16;
     }
   };
   auto load_chunk = [&](int i, unsigned at, int slot) {
@@ -182,7 +191,7 @@ __global__ void __launch_bounds__(64 * WM * WN, RESIDENT * WM * WN / 4)
   for (int x = 0; x < FN; ++x) fb[0][x] = read_b(x, 0);
 
   unsigned half = 0;     // of the scales' two places, the one in use
-  auto body = [&](unsigned g, auto step) {
+  auto body = [&](unsigned g, unsigned groups, auto step) {
     constexpr int J = decltype(step)::value;
     // stage g * 4 + J + 1 is here, for every wave, and every wave has read the one before it
     constexpr int kAfter = 2 * kLoads + (J == 1 || J == 2 ? kScaleLoads : 0);
@@ -227,19 +236,27 @@ __global__ void __launch_bounds__(64 * WM * WN, RESIDENT * WM * WN / 4)
       for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
     unsigned next_m = 0, next_n = 0;
     const bool more = tiles.get(round + 1, next_m, next_n);
+    unsigned groups = all_groups, col = tn;
+    T* part_c = c;
+    if constexpr (SPLIT) {
+      const unsigned part = part_cols.quot(tn);
+      col -= part * part_cols.d;
+      groups = min(per, all_groups - part * per);
+      part_c += static_cast<size_t>(part) * m * n;
+    }
 #pragma unroll 1
     for (unsigned g = 0; g < groups; ++g) {
       if (g + 1 == groups) aim(more, next_m, next_n);
-      body(g, Int<0>{});
-      body(g, Int<1>{});
-      body(g, Int<2>{});
-      body(g, Int<3>{});
+      body(g, groups, Int<0>{});
+      body(g, groups, Int<1>{});
+      body(g, groups, Int<2>{});
+      body(g, groups, Int<3>{});
     }
 
     unsigned l = lane;
     asm volatile("" : "+v"(l));  // what follows from the lane is computed here, not kept through the loop above
-    const unsigned row0 = (tm * WM + wm) * FM * 16, col0 = (tn * WN + wn) * FN * 16, r = l & 15, q = l >> 4;
-    T* out = c + static_cast<int64_t>(row0) * stride + col0;
+    const unsigned row0 = (tm * WM + wm) * FM * 16, col0 = (col * WN + wn) * FN * 16, r = l & 15, q = l >> 4;
+    T* out = part_c + static_cast<int64_t>(row0) * stride + col0;
     char* piece = lds + 4 * kStage + 2 * kScales + wave * kOut;
     auto leave = [&](auto store) {
 #pragma unroll
@@ -270,7 +287,7 @@ __global__ void __launch_bounds__(64 * WM * WN, RESIDENT * WM * WN / 4)
     };
     if (__builtin_amdgcn_readfirstlane(row0 + FM * 16 <= m && col0 + FN * 16 <= n)) {
       leave([&](unsigned row, unsigned col, const T* v) {
-        __builtin_memcpy(out + static_cast<int64_t>(row) * stride + col, v, 16);
+        store16(out + static_cast<int64_t>(row) * stride + col, v);
       });
     } else {
       leave([&](unsigned row, unsigned col, const T* v) {
@@ -284,6 +301,34 @@ __global__ void __launch_bounds__(64 * WM * WN, RESIDENT * WM * WN / 4)
     tm = next_m, tn = next_n, ++round;
   }
   __builtin_amdgcn_s_waitcnt(wait_imm(0, true));  // no load may arrive after the workgroup's memory is given back
+}
+
+// c = the parts' sums, added up in their order; four columns a thread.
+template <typename T>
+__global__ void __launch_bounds__(256) product_sum_kernel(const float* __restrict__ sums, unsigned parts, unsigned m,
+                                                          unsigned n, T* __restrict__ c, int64_t stride, Div quarters) {
+  const unsigned i = blockIdx.x * 256 + threadIdx.x, row = quarters.quot(i), col = (i - row * quarters.d) * 4;
+  if (row >= m) return;
+  const size_t at = static_cast<size_t>(row) * n + col, step = static_cast<size_t>(m) * n;
+  T* out = c + static_cast<int64_t>(row) * stride + col;
+  if (col + 4 <= n) {
+    f32x4 v = {0, 0, 0, 0};
+    for (unsigned p = 0; p < parts; ++p) {
+      f32x4 x;
+      __builtin_memcpy(&x, sums + p * step + at, 16);
+      v += x;
+    }
+    T o[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = Elem<T>::from_f32(v[e]);
+    __builtin_memcpy(out, o, sizeof(o));
+  } else {
+    for (unsigned e = 0; col + e < n; ++e) {
+      float v = 0;
+      for (unsigned p = 0; p < parts; ++p) v += sums[p * step + at + e];
+      out[e] = Elem<T>::from_f32(v);
+    }
+  }
 }
 
 // ---- few rows ----------------------------------------------------------------------------------
@@ -459,6 +504,28 @@ int compute_units(int dev) {
 
 constexpr int64_t kFusedRows = 16, kFewRows = 64;
 
+// Which kernel a product takes.
+struct Plan {
+  enum Shape { kFew, k256, k128, k64x128, k64 } shape;
+  unsigned parts, per;  // of k, and groups of quads a part
+};
+Plan plan(int64_t m, int64_t n, int64_t k) {
+  const int64_t groups = mx_groups(k);
+  const auto whole = static_cast<unsigned>(groups);
+  auto tiles = [&](int64_t tm, int64_t tn) { return (m + tm - 1) / tm * ((n + tn - 1) / tn); };
+  if (m <= kFewRows) return {Plan::kFew, 1, whole};
+  const int64_t big = tiles(256, 256);
+  if (big * 5 >= (big + 255) / 256 * 256 * 4 && groups > 1) return {Plan::k256, 1, whole};
+  if (tiles(128, 128) >= 205) return {Plan::k128, 1, whole};
+  if (n > 64 && tiles(64, 128) >= 205) return {Plan::k64x128, 1, whole};
+  const int64_t small = tiles(64, 64);
+  if (small <= 128 && groups >= 16) {
+    const int64_t parts = std::min<int64_t>(256 / small, groups / 4), per = (groups + parts - 1) / parts;
+    return {Plan::k64, static_cast<unsigned>((groups + per - 1) / per), static_cast<unsigned>(per)};
+  }
+  return {Plan::k64, 1, whole};
+}
+
 void check_product(int64_t m, int64_t n, int64_t k, int64_t stride) {
   require(m >= 0 && n >= 0 && k >= 1, "mx: m and n must be >= 0 and k >= 1");
   require(mx_fits(m, k) && mx_fits(n, k) && ((m + 15) / 16) * ((n + 15) / 16) < (1ll << 28),
@@ -473,14 +540,15 @@ size_t round16(size_t b) { return (b + 15) / 16 * 16; }
 
 using namespace mx;
 
-size_t mx_product_workspace(int, int64_t m, int64_t n, int64_t k) {
+size_t mx_product_workspace(int64_t m, int64_t n, int64_t k) {
   check_product(m, n, k, n);
-  return 0;
+  const Plan p = plan(m, n, k);
+  return p.parts > 1 ? static_cast<size_t>(p.parts) * m * n * 4 : 0;
 }
 
 void launch_mx_product(int dev, const void* a_codes, const void* a_scales, const void* b_codes, const void* b_scales,
-                       int64_t m, int64_t n, int64_t k, void* c, const std::string& dtype, int64_t stride, void*,
-                       size_t, void* stream) {
+                       int64_t m, int64_t n, int64_t k, void* c, const std::string& dtype, int64_t stride,
+                       void* workspace, size_t workspace_bytes, void* stream) {
   const Type t = type_of(dtype, "mx_product: dtype must be bf16|f16|f32");
   check_product(m, n, k, stride);
   if (m == 0 || n == 0) return;
@@ -488,44 +556,57 @@ void launch_mx_product(int dev, const void* a_codes, const void* a_scales, const
   require(aligned(a_codes, 16) && aligned(b_codes, 16) && aligned(a_scales, 16) && aligned(b_scales, 16) &&
               aligned(c, size_of(t)),
           "mx_product: codes and scales aligned to 16 bytes, the result to its type");
+  const size_t need = mx_product_workspace(m, n, k);
+  require(need == 0 || (workspace && workspace_bytes >= need && aligned(workspace, 16)),
+          "mx_product: needs a workspace of mx_product_workspace bytes, aligned to 16");
   OnDevice on(dev);
+  auto s = static_cast<hipStream_t>(stream);
+  const Plan p = plan(m, n, k);
+  const auto um = static_cast<unsigned>(m), un = static_cast<unsigned>(n);
   with_type(t, [&](auto e) {
     using T = decltype(e);
-    auto run = [&](auto kernel, int tile_m, int tile_n, int waves, int resident) {
-      const unsigned tn = static_cast<unsigned>((n + tile_n - 1) / tile_n), tm = static_cast<unsigned>((m + tile_m - 1) / tile_m);
-      const unsigned total = tm * tn, grid = std::min((total + 7) / 8 * 8, static_cast<unsigned>(compute_units(dev) * resident));
-      hipLaunchKernelGGL(kernel, dim3(grid), dim3(64 * waves), 0, static_cast<hipStream_t>(stream),
-                         static_cast<const char*>(a_codes), static_cast<const char*>(a_scales),
-                         static_cast<const char*>(b_codes), static_cast<const char*>(b_scales),
-                         static_cast<unsigned>(m), static_cast<unsigned>(n), static_cast<unsigned>(mx_quads(k)),
-                         static_cast<T*>(c), stride, Tiles(tm, tn));
+    auto out = static_cast<T*>(c);
+    auto run = [&](auto kernel, auto* to, int64_t to_stride, int tile_m, int tile_n, int waves, int resident) {
+      const unsigned cols = (un + tile_n - 1) / tile_n, rows = (um + tile_m - 1) / tile_m, total = rows * cols * p.parts;
+      const unsigned grid = std::min((total + 7) / 8 * 8, static_cast<unsigned>(compute_units(dev) * resident));
+      hipLaunchKernelGGL(kernel, dim3(grid), dim3(64 * waves), 0, s, static_cast<const char*>(a_codes),
+                         static_cast<const char*>(a_scales), static_cast<const char*>(b_codes),
+                         static_cast<const char*>(b_scales), um, un, static_cast<unsigned>(mx_quads(k)), to, to_stride,
+                         Tiles(rows, cols * p.parts), Div(cols), p.per);
     };
-    if (m <= kFewRows) {
-      const QuantizedRows x{static_cast<const char*>(a_codes), static_cast<const char*>(a_scales),
-                            static_cast<unsigned>(mx_quads(k)), static_cast<unsigned>(mx_groups(k)),
-                            static_cast<unsigned>(mx_row_blocks(m))};
-      auto s = static_cast<hipStream_t>(stream);
-      auto out = static_cast<T*>(c);
-      if (m <= 16) launch_few_rows<T, 1, 1, 2>(x, b_codes, b_scales, m, n, k, out, stride, s);
-      else if (m <= 32) launch_few_rows<T, 2, 2, 2>(x, b_codes, b_scales, m, n, k, out, stride, s);
-      else launch_few_rows<T, 4, 2, 2>(x, b_codes, b_scales, m, n, k, out, stride, s);
-    } else if (m > 1024 && n > 1024) { const char* v = getenv("MXV"); int w = v ? atoi(v) : 0;
-      if (w == 0) run(product_tile_kernel<T, 8, 4, 2, 4, 1>, 256, 256, 8, 1);
-      else if (w == 1) run(product_tile_kernel<T, 8, 8, 2, 2, 1>, 256, 256, 4, 1);
-      else if (w == 2) run(product_tile_kernel<T, 4, 8, 4, 2, 1>, 256, 256, 8, 1);
-      else if (w == 3) run(product_tile_kernel<T, 4, 4, 2, 2, 2>, 128, 128, 4, 2);
-      else if (w == 4) run(product_tile_kernel<T, 8, 4, 2, 2, 1>, 256, 128, 4, 1);
-      else run(product_tile_kernel<T, 4, 4, 4, 2, 1>, 256, 128, 8, 1); }
-    else if (m > 64 && n > 64) run(product_tile_kernel<T, 4, 4, 2, 2, 2>, 128, 128, 4, 2);
-    else run(product_tile_kernel<T, 2, 2, 2, 2, 2>, 64, 64, 4, 2);
+    switch (p.shape) {
+      case Plan::kFew: {
+        const QuantizedRows x{static_cast<const char*>(a_codes), static_cast<const char*>(a_scales),
+                              static_cast<unsigned>(mx_quads(k)), static_cast<unsigned>(mx_groups(k)),
+                              static_cast<unsigned>(mx_row_blocks(m))};
+        if (m <= 16) launch_few_rows<T, 1, 1, 2>(x, b_codes, b_scales, m, n, k, out, stride, s);
+        else if (m <= 32) launch_few_rows<T, 2, 2, 2>(x, b_codes, b_scales, m, n, k, out, stride, s);
+        else launch_few_rows<T, 4, 2, 2>(x, b_codes, b_scales, m, n, k, out, stride, s);
+        break;
+      }
+      case Plan::k256: run(product_tile_kernel<T, 8, 4, 2, 4, 1>, out, stride, 256, 256, 8, 1); break;
+      case Plan::k128: run(product_tile_kernel<T, 4, 4, 2, 2, 2>, out, stride, 128, 128, 4, 2); break;
+      case Plan::k64x128: run(product_tile_kernel<T, 2, 4, 2, 2, 2>, out, stride, 64, 128, 4, 2); break;
+      case Plan::k64:
+        if (p.parts == 1) {
+          run(product_tile_kernel<T, 2, 2, 2, 2, 3>, out, stride, 64, 64, 4, 3);
+        } else {
+          auto sums = static_cast<float*>(workspace);
+          run(product_tile_kernel<float, 2, 2, 2, 2, 3, true>, sums, n, 64, 64, 4, 3);
+          const unsigned quarters = (un + 3) / 4;
+          hipLaunchKernelGGL(product_sum_kernel<T>, dim3(static_cast<unsigned>((m * quarters + 255) / 256)), dim3(256), 0, s,
+                             sums, p.parts, um, un, out, stride, Div(quarters));
+        }
+        break;
+    }
   });
   check(hipGetLastError(), "mx_product");
 }
 
-size_t mx_linear_workspace(int dev, int64_t m, int64_t n, int64_t k) {
+size_t mx_linear_workspace(int64_t m, int64_t n, int64_t k) {
   check_product(m, n, k, n);
   if (m <= kFusedRows) return 0;
-  return round16(static_cast<size_t>(mx_codes_bytes(m, k) + mx_scales_bytes(m, k))) + mx_product_workspace(dev, m, n, k);
+  return round16(static_cast<size_t>(mx_codes_bytes(m, k) + mx_scales_bytes(m, k))) + mx_product_workspace(m, n, k);
 }
 
 void launch_mx_linear(int dev, const void* x, const std::string& dtype, int64_t x_stride, const void* w_codes,
@@ -555,7 +636,7 @@ void launch_mx_linear(int dev, const void* x, const std::string& dtype, int64_t 
     check(hipGetLastError(), "mx_linear");
     return;
   }
-  require(workspace && workspace_bytes >= mx_linear_workspace(dev, m, n, k), "mx_linear: workspace too small");
+  require(workspace && workspace_bytes >= mx_linear_workspace(m, n, k), "mx_linear: workspace too small");
   require(aligned(workspace, 16), "mx_linear: workspace aligned to 16 bytes");
   auto codes = static_cast<char*>(workspace);
   auto scales = codes + mx_codes_bytes(m, k);

@@ -180,9 +180,7 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const char* __restrict_
     }
     T* o = out + static_cast<int64_t>(row) * stride + k0;
     if (k0 + static_cast<int>(kPer) <= k) {
-      // written once and larger than what it came from: past the caches
-      struct __attribute__((packed, aligned(sizeof(T)))) Out { u32x4 q; };
-      __builtin_nontemporal_store(__builtin_bit_cast(u32x4, v), &reinterpret_cast<Out*>(o)->q);
+      store16(o, v);
     } else {
 #pragma unroll
       for (unsigned j = 0; j < kPer; ++j)

@@ -195,7 +195,7 @@ def matmul(a: MxTensor, b: MxTensor, dtype=torch.bfloat16):
     c = torch.empty(a.rows, b.rows, dtype=dtype, device=a.device)
     if c.numel():
         h, dev = hip(), a.device.index
-        need = h.mx_product_workspace(dev, a.rows, b.rows, a.k)
+        need = h.mx_product_workspace(a.rows, b.rows, a.k)
         ws = torch.empty(need, dtype=torch.uint8, device=a.device) if need else None
         h.mx_product(dev, a._codes, a._scales, b._codes, b._scales, a.rows, b.rows, a.k, c.data_ptr(), DTYPES[dtype],
                      b.rows, ws.data_ptr() if need else 0, need, _stream(a.device))
@@ -216,7 +216,7 @@ def linear(x, w: MxTensor):
     y = torch.empty(*x.shape[:-1], n, dtype=x.dtype, device=x.device)
     if y.numel():
         h, dev = hip(), x.device.index
-        need = h.mx_linear_workspace(dev, m, n, w.k)
+        need = h.mx_linear_workspace(m, n, w.k)
         ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
         h.mx_linear(dev, x2.data_ptr(), DTYPES[x.dtype], _row_stride(x2), w._codes, w._scales, m, n, w.k, y.data_ptr(),
                     n, ws.data_ptr() if need else 0, need, _stream(x.device))

@@ -193,7 +193,7 @@ PRODUCTS = [(1, 1, 1), (1, 16, 32), (1, 1000, 4096), (2, 33, 64), (7, 130, 129),
             (17, 48, 640), (31, 1411, 256), (33, 65, 300), (64, 64, 128), (65, 257, 1025), (100, 100, 100),
             (128, 128, 256), (129, 300, 384), (200, 1000, 2500), (256, 256, 256), (257, 511, 768), (300, 260, 130),
             (512, 512, 1152), (513, 1030, 2048), (777, 1411, 2999), (1024, 2048, 640), (2100, 1100, 300), (1, 70000, 96),
-            (5000, 3, 200), (3, 5, 100000), (40, 40, 20000)]
+            (5000, 3, 200), (3, 5, 100000), (40, 40, 20000), (70, 66, 9000), (130, 200, 8192), (500, 300, 33000), (300, 20, 12345)]
 
 
 @pytest.mark.parametrize("m,n,k", PRODUCTS)
@@ -248,7 +248,7 @@ def test_layouts_of_results_leave_their_surroundings_alone(mx):
         a, b = values(m, k, F32, 1), values(n, k, F32, 2)
         qa, qb = mx.quantize(a), mx.quantize(b)
         out = torch.full((m + 2, n + 13), 5.0, dtype=dt, device="cuda")
-        need = H.mx_product_workspace(0, m, n, k)
+        need = H.mx_product_workspace(m, n, k)
         ws = torch.empty(max(need, 1), dtype=torch.uint8, device="cuda")
         H.mx_product(0, qa.codes.data_ptr(), qa.scales.data_ptr(), qb.codes.data_ptr(), qb.scales.data_ptr(), m, n, k,
                      out[1:, 3:].data_ptr(), mx.DTYPES[dt], n + 13, ws.data_ptr(), need, s)
@@ -381,7 +381,7 @@ def test_two_layers_trained_and_served_together(mx):
         assert_product(mx.linear(hs, q2), ref_round(hs), ref_round(n2))
 
 
-@pytest.mark.parametrize("m,n,k", [(1, 1000, 4096), (8, 200, 30000), (40, 300, 5000), (200, 500, 3000), (600, 700, 500)])
+@pytest.mark.parametrize("m,n,k", [(1, 1000, 4096), (8, 200, 30000), (40, 300, 5000), (200, 500, 3000), (600, 700, 500), (100, 300, 16384)])
 def test_results_repeat_bit_for_bit(mx, m, n, k):
     x, w = values(m, k, BF16, 1), mx.quantize(values(n, k, BF16, 2))
     first = mx.linear(x, w)
@@ -389,7 +389,7 @@ def test_results_repeat_bit_for_bit(mx, m, n, k):
         assert torch.equal(mx.linear(x, w), first)
 
 
-@pytest.mark.parametrize("m,n,k", [(1, 1000, 4096), (8, 200, 30000), (40, 300, 5000), (300, 500, 700)])
+@pytest.mark.parametrize("m,n,k", [(1, 1000, 4096), (8, 200, 30000), (40, 300, 5000), (300, 500, 700), (100, 130, 9000)])
 def test_two_streams_and_two_graphs(mx, m, n, k):
     """Calls on two streams at once and two captured graphs replayed in turn with eager work between
     them: each has workspaces of its own."""
