@@ -95,18 +95,60 @@ __device__ __forceinline__ unsigned codes8(const unsigned* w, float s) {
 }
 
 // Eight elements of a row from column k0 on as words, zeros from column k on. Rows start where the
-// caller's stride puts them, so the 16 bytes need not be aligned (one unaligned load).
+// caller's stride puts them, so the 16 bytes need not be aligned. A branch a lane would make the
+// compiler wait for each load by itself, so how to load is chosen for a wave: all within the row; up to
+// the row's end, reading its last 16 bytes instead and shifting them into place; or a row of fewer.
+enum class Reach { whole, end, tiny };
 template <typename T>
+__device__ __forceinline__ Reach reach(int end, int k) {  // end: past the wave's last column
+  return end <= k ? Reach::whole : k >= 16 / static_cast<int>(sizeof(T)) ? Reach::end : Reach::tiny;
+}
+// v's bytes from `n` on, zeros after them
+__device__ __forceinline__ void shift16(unsigned* v, unsigned n) {
+  uint64_t lo = v[0] | static_cast<uint64_t>(v[1]) << 32, hi = v[2] | static_cast<uint64_t>(v[3]) << 32;
+  const unsigned bits = n % 8 * 8;
+  if (n >= 16) hi = 0;
+  if (n >= 8) lo = hi, hi = 0;
+  lo = lo >> bits | hi << 1 << (63 - bits);
+  hi >>= bits;
+  v[0] = static_cast<unsigned>(lo), v[1] = static_cast<unsigned>(lo >> 32);
+  v[2] = static_cast<unsigned>(hi), v[3] = static_cast<unsigned>(hi >> 32);
+}
+template <Reach R, typename T>
 __device__ __forceinline__ void load8(const T* __restrict__ row, int k0, int k, unsigned* w) {
-  constexpr int N = 8 / Elem<T>::kPerWord;
-  if (k0 + 8 <= k) {
-    __builtin_memcpy(w, row + k0, N * 4);
-  } else {
-    T v[8];
+  constexpr int kPer = 16 / sizeof(T);  // elements of 16 bytes
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = k0 + j < k ? row[k0 + j] : T{};
-    __builtin_memcpy(w, v, N * 4);
+  for (int h = 0; h < 8 / kPer; ++h) {
+    unsigned* v = w + h * 4;
+    const int c = k0 + h * kPer;
+    if constexpr (R == Reach::whole) {
+      __builtin_memcpy(v, row + c, 16);
+    } else if constexpr (R == Reach::end) {
+      const int from = min(c, k - kPer);
+      __builtin_memcpy(v, row + from, 16);
+      shift16(v, static_cast<unsigned>(min(c - from, kPer)) * sizeof(T));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[i] = 0;
+#pragma unroll
+        for (unsigned e = 0; e < 4 / sizeof(T); ++e) {
+          const int at = c + i * (4 / static_cast<int>(sizeof(T))) + static_cast<int>(e);
+          unsigned bits = 0;
+          __builtin_memcpy(&bits, row + min(at, k - 1), sizeof(T));
+          v[i] |= (at < k ? bits : 0u) << (e * 8 * sizeof(T));
+        }
+      }
+    }
   }
+}
+// f(reach) with the reach as a constant
+template <typename T, typename F>
+__device__ __forceinline__ void with_reach(int end, int k, F f) {
+  const Reach r = reach<T>(end, k);
+  if (r == Reach::whole) f(std::integral_constant<Reach, Reach::whole>{});
+  else if (r == Reach::end) f(std::integral_constant<Reach, Reach::end>{});
+  else f(std::integral_constant<Reach, Reach::tiny>{});
 }
 
 // 16 bytes written once, past the caches (6.3 TB/s where plain stores came to 3.5), aligned or not.
@@ -139,6 +181,28 @@ struct Div {
   }
   __device__ __forceinline__ unsigned quot(unsigned x) const {
     return d == 1 ? x : static_cast<unsigned>((static_cast<uint64_t>(x) * m) >> 32) >> s;
+  }
+};
+
+// A matrix's tiles in the order in which workgroups take them: bands of H rows of tiles, down each column
+// of a band. Workgroups run on the eight XCDs in turn, and each XCD takes a run of neighbours in this
+// order, so that what neighbours share meets in one cache.
+template <unsigned H>
+struct Tiles {
+  unsigned rows, cols, total;
+  Div band, last;  // tiles of a band; rows of the last band
+  Tiles(unsigned r, unsigned c) : rows(r), cols(c), total(r * c), band(H * c), last((r + H - 1) % H + 1) {}
+  unsigned whole_grid() const { return (total + 7) / 8 * 8; }
+  // tile `r` of this workgroup; false if it has none
+  __device__ __forceinline__ bool get(unsigned r, unsigned& row, unsigned& col) const {
+    const unsigned first = r * gridDim.x, place = blockIdx.x / 8;
+    const unsigned count = first < total ? min(total - first, gridDim.x) : 0, per = (count + 7) / 8;
+    const unsigned p = blockIdx.x % 8 * per + place, b = band.quot(first + p), in = first + p - b * band.d;
+    const bool whole = b * H + H <= rows;
+    col = whole ? in / H : last.quot(in);
+    row = b * H + in - col * (whole ? H : last.d);
+    row = __builtin_amdgcn_readfirstlane(row), col = __builtin_amdgcn_readfirstlane(col);
+    return place < per && p < count;
   }
 };
 

@@ -35,26 +35,6 @@ __device__ __forceinline__ void load_lds(Buffer b, unsigned offset, unsigned uni
 template <int S>
 using Int = std::integral_constant<int, S>;
 
-// The tiles of a product in the order in which the workgroups take them: bands of eight rows of tiles,
-// down each column of a band. Workgroups run on the eight XCDs in turn, and each XCD takes a run of
-// neighbours in this order (with 32 CUs, 8 x 4 tiles), so that its cache sees each operand's rows once.
-struct Tiles {
-  unsigned rows, cols, total;
-  Div band, last;  // tiles of a band; rows of the last band
-  Tiles(unsigned r, unsigned c) : rows(r), cols(c), total(r * c), band(8 * c), last((r + 7) % 8 + 1) {}
-  // tile `r` of this workgroup; false if it has none
-  __device__ __forceinline__ bool get(unsigned r, unsigned& row, unsigned& col) const {
-    const unsigned first = r * gridDim.x, place = blockIdx.x / 8;
-    const unsigned count = first < total ? min(total - first, gridDim.x) : 0, per = (count + 7) / 8;
-    const unsigned p = blockIdx.x % 8 * per + place, b = band.quot(first + p), in = first + p - b * band.d;
-    const bool whole = b * 8 + 8 <= rows;
-    col = whole ? in / 8 : last.quot(in);
-    row = b * 8 + in - col * (whole ? 8 : last.d);
-    row = __builtin_amdgcn_readfirstlane(row), col = __builtin_amdgcn_readfirstlane(col);
-    return place < per && p < count;
-  }
-};
-
 // The order of a stage's work in a wave: FM x FN matrix instructions, row after row, and between them,
 // evenly, the next stages' loads (kLoad), and the next stage's operands from LDS: b's (kB), a's last TAIL
 // rows (kTail), for both of which there are two sets of registers, and a's other rows (kA), each into the
@@ -103,7 +83,7 @@ template <typename T, int FM, int FN, int WM, int WN, int RESIDENT, bool SPLIT =
 __global__ void __launch_bounds__(64 * WM * WN, RESIDENT * WM * WN / 4)
     product_tile_kernel(const char* __restrict__ ac, const char* __restrict__ as, const char* __restrict__ bc,
                         const char* __restrict__ bs, unsigned m, unsigned n, unsigned quads, T* __restrict__ c,
-                        int64_t stride, Tiles tiles, Div part_cols, unsigned per) {
+                        int64_t stride, Tiles<8> tiles, Div part_cols, unsigned per) {
   constexpr int TM = FM * WM, TN = FN * WN, kChunks = TM + TN, kLoads = kChunks / (WM * WN);
   constexpr int kScaleLoads = kChunks >= 4 * WM * WN ? kChunks / (4 * WM * WN) : 1;
   constexpr int kStage = kChunks * 1024, kScales = kChunks * 256;
@@ -336,13 +316,12 @@ __global__ void __launch_bounds__(256) product_sum_kernel(const float* __restric
 // results a row of x), its waves whole groups of quads in turn, straight from memory to registers,
 // U groups a wave in flight; the waves' sums meet in LDS in a fixed order. Sources of x: rows
 // quantised before, or plain rows that each wave quantises for its own groups.
-constexpr int kWaves = 8;
-
 struct QuantizedRows {
   const char* codes;
   const char* scales;
   unsigned quads, groups, row_blocks;
   struct Raw {};
+  static constexpr bool kFirst = false;
   static constexpr int kLds = 16;
   template <int FM, bool FULL>
   __device__ __forceinline__ void load(unsigned g, unsigned nq, unsigned lane, Raw&, u32x4 (&x)[4][FM], unsigned (&sx)[FM]) const {
@@ -362,7 +341,7 @@ struct QuantizedRows {
   __device__ __forceinline__ void finish(const Raw&, unsigned, char*, u32x4 (&)[4][FM], unsigned (&)[FM]) const {}
 };
 
-// Up to ROWS plain rows (ROWS <= 16): eight elements a lane of one row after the other, 16 lanes a quad,
+// Up to ROWS plain rows: eight elements a lane of one row after the other, 16 lanes a quad,
 // as the quantising kernel does; the codes change lanes in the wave's own piece of LDS. Rows of the
 // operand from ROWS on repeat the last one.
 template <typename X, int ROWS>
@@ -375,12 +354,16 @@ struct PlainRows {
   struct Raw {
     unsigned w[ROWS][kWords];
   };
+  static constexpr bool kFirst = true;
   static constexpr int kLds = ROWS * 256 + 64 * ROWS;
   template <int FM, bool FULL>
   __device__ __forceinline__ void load(unsigned g, unsigned, unsigned lane, Raw& raw, u32x4 (&)[4][FM], unsigned (&)[FM]) const {
+    with_reach<X>(static_cast<int>(g * 512 + 512), k, [&](auto how) {
 #pragma unroll
-    for (unsigned r = 0; r < ROWS; ++r)
-      load8(x + static_cast<int64_t>(min(r, m - 1)) * stride, static_cast<int>(g * 512 + lane * 8), k, raw.w[r]);
+      for (unsigned r = 0; r < ROWS; ++r)
+        load8<decltype(how)::value>(x + static_cast<int64_t>(min(r, m - 1)) * stride, static_cast<int>(g * 512 + lane * 8), k,
+                                    raw.w[r]);
+    });
   }
   template <int FM>
   __device__ __forceinline__ void finish(const Raw& raw, unsigned lane, char* lds, u32x4 (&x)[4][FM], unsigned (&sx)[FM]) const {
@@ -410,7 +393,7 @@ struct PlainRows {
   }
 };
 
-template <typename T, typename Source, int FM, int R, int U>
+template <typename T, typename Source, int FM, int R, int U, int kWaves>
 __global__ void __launch_bounds__(64 * kWaves) product_few_rows_kernel(Source source, const char* __restrict__ bc,
                                                                        const char* __restrict__ bs, unsigned m, unsigned n,
                                                                        unsigned quads, T* __restrict__ c, int64_t stride) {
@@ -427,8 +410,13 @@ __global__ void __launch_bounds__(64 * kWaves) product_few_rows_kernel(Source so
     u32x4 x[N][4][FM], w[N][R][4];
     unsigned sx[N][FM], sw[N][R];
     const unsigned nq = FULL ? 4 : quads - g0 * 4;
+    auto load_x = [&] {
 #pragma unroll
-    for (int u = 0; u < N; ++u) source.template load<FM, FULL>(g0 + u * kWaves, nq, lane, raw[u], x[u], sx[u]);
+      for (int u = 0; u < N; ++u) source.template load<FM, FULL>(g0 + u * kWaves, nq, lane, raw[u], x[u], sx[u]);
+    };
+    // Loads come back in order. Plain rows come first, to be quantised while the weights are on their way;
+    // quantised ones come last: there are up to twice as many of them, and the weights have further to go.
+    if constexpr (Source::kFirst) load_x();
 #pragma unroll
     for (int u = 0; u < N; ++u)
 #pragma unroll
@@ -443,6 +431,7 @@ __global__ void __launch_bounds__(64 * kWaves) product_few_rows_kernel(Source so
           else
             w[u][r][q] = u32x4{0, 0, 0, 0};
       }
+    if constexpr (!Source::kFirst) load_x();
 #pragma unroll
     for (int u = 0; u < N; ++u) {
       source.template finish<FM>(raw[u], lane, lds + wave * Source::kLds, x[u], sx[u]);
@@ -483,11 +472,16 @@ __global__ void __launch_bounds__(64 * kWaves) product_few_rows_kernel(Source so
 }
 
 template <typename T, int FM, int R, int U, typename Source>
-void launch_few_rows(Source source, const void* bc, const void* bs, int64_t m, int64_t n, int64_t k, T* c,
-                     int64_t stride, hipStream_t s) {
-  hipLaunchKernelGGL((product_few_rows_kernel<T, Source, FM, R, U>), dim3(static_cast<unsigned>((n + 16 * R - 1) / (16 * R))),
-                     dim3(64 * kWaves), 0, s, source, static_cast<const char*>(bc), static_cast<const char*>(bs),
-                     static_cast<unsigned>(m), static_cast<unsigned>(n), static_cast<unsigned>(mx_quads(k)), c, stride);
+void few_rows(Source source, const void* bc, const void* bs, int64_t m, int64_t n, int64_t k, T* c, int64_t stride,
+              hipStream_t s) {
+  auto run = [&](auto kernel, int waves) {
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>((n + 16 * R - 1) / (16 * R))), dim3(64 * waves), 0, s, source,
+                       static_cast<const char*>(bc), static_cast<const char*>(bs), static_cast<unsigned>(m),
+                       static_cast<unsigned>(n), static_cast<unsigned>(mx_quads(k)), c, stride);
+  };
+  // no more waves than groups of quads
+  if (mx_groups(k) <= 4) run(product_few_rows_kernel<T, Source, FM, R, 1, 4>, 4);
+  else run(product_few_rows_kernel<T, Source, FM, R, U, 8>, 8);
 }
 
 // Compute units, asked for once a device (a multiple of eight: whole XCDs).
@@ -502,8 +496,10 @@ int compute_units(int dev) {
   return n;
 }
 
-constexpr int64_t kFusedRows = 16, kFewRows = 64;
+constexpr int64_t kFewRows = 64;
+constexpr int kComputeUnits = 256;  // what the choices between kernels are made for
 
+constexpr int kEnough = kComputeUnits * 4 / 5;  // tiles that fill the chip
 // Which kernel a product takes.
 struct Plan {
   enum Shape { kFew, k256, k128, k64x128, k64 } shape;
@@ -513,14 +509,14 @@ Plan plan(int64_t m, int64_t n, int64_t k) {
   const int64_t groups = mx_groups(k);
   const auto whole = static_cast<unsigned>(groups);
   auto tiles = [&](int64_t tm, int64_t tn) { return (m + tm - 1) / tm * ((n + tn - 1) / tn); };
-  if (m <= kFewRows) return {Plan::kFew, 1, whole};
+  if (m <= 32 || (m <= kFewRows && tiles(64, 64) < 192)) return {Plan::kFew, 1, whole};
   const int64_t big = tiles(256, 256);
-  if (big * 5 >= (big + 255) / 256 * 256 * 4 && groups > 1) return {Plan::k256, 1, whole};
-  if (tiles(128, 128) >= 205) return {Plan::k128, 1, whole};
-  if (n > 64 && tiles(64, 128) >= 205) return {Plan::k64x128, 1, whole};
+  if (big * 5 >= (big + kComputeUnits - 1) / kComputeUnits * kComputeUnits * 4 && groups > 1) return {Plan::k256, 1, whole};
+  if (tiles(128, 128) >= kEnough) return {Plan::k128, 1, whole};
+  if (n > 64 && tiles(64, 128) >= kEnough) return {Plan::k64x128, 1, whole};
   const int64_t small = tiles(64, 64);
-  if (small <= 128 && groups >= 16) {
-    const int64_t parts = std::min<int64_t>(256 / small, groups / 4), per = (groups + parts - 1) / parts;
+  if (small * 2 <= kComputeUnits && groups >= 16) {
+    const int64_t parts = std::min<int64_t>(kComputeUnits / small, groups / 4), per = (groups + parts - 1) / parts;
     return {Plan::k64, static_cast<unsigned>((groups + per - 1) / per), static_cast<unsigned>(per)};
   }
   return {Plan::k64, 1, whole};
@@ -531,6 +527,13 @@ void check_product(int64_t m, int64_t n, int64_t k, int64_t stride) {
   require(mx_fits(m, k) && mx_fits(n, k) && ((m + 15) / 16) * ((n + 15) / 16) < (1ll << 28),
           "mx: a product's sizes are beyond its limits (mx.h)");
   require(stride >= n || m <= 1, "mx: stride must be at least n");
+}
+
+// Whether a linear layer's rows are quantised by the workgroups that multiply them, each for itself, or
+// once by a launch before. The launch costs 2.6 us; on the way, 64 Ki elements a compute unit cost 2 us.
+bool quantise_on_the_way(int64_t m, int64_t n, int64_t k) {
+  const int64_t blocks = (n + 15) / 16, workgroups = m > 4 && blocks > kComputeUnits ? (blocks + 1) / 2 : blocks;
+  return m <= 8 && m * k * ((workgroups + kComputeUnits - 1) / kComputeUnits) <= (1 << 17);
 }
 
 size_t round16(size_t b) { return (b + 15) / 16 * 16; }
@@ -572,16 +575,19 @@ void launch_mx_product(int dev, const void* a_codes, const void* a_scales, const
       hipLaunchKernelGGL(kernel, dim3(grid), dim3(64 * waves), 0, s, static_cast<const char*>(a_codes),
                          static_cast<const char*>(a_scales), static_cast<const char*>(b_codes),
                          static_cast<const char*>(b_scales), um, un, static_cast<unsigned>(mx_quads(k)), to, to_stride,
-                         Tiles(rows, cols * p.parts), Div(cols), p.per);
+                         Tiles<8>(rows, cols * p.parts), Div(cols), p.per);
     };
     switch (p.shape) {
       case Plan::kFew: {
         const QuantizedRows x{static_cast<const char*>(a_codes), static_cast<const char*>(a_scales),
                               static_cast<unsigned>(mx_quads(k)), static_cast<unsigned>(mx_groups(k)),
                               static_cast<unsigned>(mx_row_blocks(m))};
-        if (m <= 16) launch_few_rows<T, 1, 1, 2>(x, b_codes, b_scales, m, n, k, out, stride, s);
-        else if (m <= 32) launch_few_rows<T, 2, 2, 2>(x, b_codes, b_scales, m, n, k, out, stride, s);
-        else launch_few_rows<T, 4, 2, 2>(x, b_codes, b_scales, m, n, k, out, stride, s);
+        const bool narrow = n <= 16 * kComputeUnits;  // a row block a workgroup fills the chip better than two
+        if (m <= 16) few_rows<T, 1, 1, 2>(x, b_codes, b_scales, m, n, k, out, stride, s);
+        else if (m <= 32 && narrow) few_rows<T, 2, 1, 2>(x, b_codes, b_scales, m, n, k, out, stride, s);
+        else if (m <= 32) few_rows<T, 2, 2, 2>(x, b_codes, b_scales, m, n, k, out, stride, s);
+        else if (narrow) few_rows<T, 4, 1, 1>(x, b_codes, b_scales, m, n, k, out, stride, s);
+        else few_rows<T, 4, 2, 2>(x, b_codes, b_scales, m, n, k, out, stride, s);
         break;
       }
       case Plan::k256: run(product_tile_kernel<T, 8, 4, 2, 4, 1>, out, stride, 256, 256, 8, 1); break;
@@ -605,7 +611,7 @@ void launch_mx_product(int dev, const void* a_codes, const void* a_scales, const
 
 size_t mx_linear_workspace(int64_t m, int64_t n, int64_t k) {
   check_product(m, n, k, n);
-  if (m <= kFusedRows) return 0;
+  if (quantise_on_the_way(m, n, k)) return 0;
   return round16(static_cast<size_t>(mx_codes_bytes(m, k) + mx_scales_bytes(m, k))) + mx_product_workspace(m, n, k);
 }
 
@@ -619,7 +625,7 @@ void launch_mx_linear(int dev, const void* x, const std::string& dtype, int64_t 
   require(x && w_codes && w_scales && y, "mx_linear: null pointer");
   require(aligned(x, size_of(t)) && aligned(y, size_of(t)) && aligned(w_codes, 16) && aligned(w_scales, 16),
           "mx_linear: x and y aligned to their type, codes and scales to 16 bytes");
-  if (m <= kFusedRows) {
+  if (quantise_on_the_way(m, n, k)) {
     OnDevice on(dev);
     auto s = static_cast<hipStream_t>(stream);
     with_type(t, [&](auto e) {
@@ -628,10 +634,10 @@ void launch_mx_linear(int dev, const void* x, const std::string& dtype, int64_t 
       auto out = static_cast<T*>(y);
       const auto rows = static_cast<unsigned>(m);
       const int len = static_cast<int>(k);
-      if (m == 1) launch_few_rows<T, 1, 1, 2>(PlainRows<T, 1>{px, x_stride, rows, len}, w_codes, w_scales, m, n, k, out, y_stride, s);
-      else if (m <= 4) launch_few_rows<T, 1, 1, 2>(PlainRows<T, 4>{px, x_stride, rows, len}, w_codes, w_scales, m, n, k, out, y_stride, s);
-      else if (m <= 8) launch_few_rows<T, 1, 2, 1>(PlainRows<T, 8>{px, x_stride, rows, len}, w_codes, w_scales, m, n, k, out, y_stride, s);
-      else launch_few_rows<T, 1, 2, 1>(PlainRows<T, 16>{px, x_stride, rows, len}, w_codes, w_scales, m, n, k, out, y_stride, s);
+      if (m == 1) few_rows<T, 1, 1, 2>(PlainRows<T, 1>{px, x_stride, rows, len}, w_codes, w_scales, m, n, k, out, y_stride, s);
+      else if (m <= 4) few_rows<T, 1, 1, 2>(PlainRows<T, 4>{px, x_stride, rows, len}, w_codes, w_scales, m, n, k, out, y_stride, s);
+      else if (n <= 16 * kComputeUnits) few_rows<T, 1, 1, 1>(PlainRows<T, 8>{px, x_stride, rows, len}, w_codes, w_scales, m, n, k, out, y_stride, s);
+      else few_rows<T, 1, 2, 1>(PlainRows<T, 8>{px, x_stride, rows, len}, w_codes, w_scales, m, n, k, out, y_stride, s);
     });
     check(hipGetLastError(), "mx_linear");
     return;

@@ -15,130 +15,131 @@ struct Piece {
   __device__ static unsigned at(unsigned quad, unsigned block, unsigned row, unsigned w) {
     return quad * 256 + block * 64 + ((row + block + 4 * quad) & 15) * 4 + w;
   }
+  // A wave's 512 elements of a row, eight a lane: 16 lanes a quad, so four lanes share a block.
+  template <typename T>
+  __device__ __forceinline__ void put(const unsigned* w, unsigned row, unsigned lane) {
+    const unsigned quad = lane >> 4, block = (lane >> 2) & 3;
+    unsigned m = 0;
+#pragma unroll
+    for (int i = 0; i < 8 / Elem<T>::kPerWord; ++i) m = Elem<T>::amax(m, w[i]);
+    m = Elem<T>::amax_f32(m);
+    m = max(m, dpp<kXor1>(m));
+    m = max(m, dpp<kXor2>(m));
+    const unsigned byte = scale_byte(m);
+    codes[at(quad, block, row, lane & 3)] = byte == 255 ? 0u : codes8<T>(w, scale_of(byte));
+    if ((lane & 3) == 0) scales[(block * 16 + row) * 4 + quad] = static_cast<unsigned char>(byte);
+  }
+  // By 256 threads, to row block rb and group g.
+  __device__ __forceinline__ void store(char* out, char* out_scales, unsigned rb, unsigned g, unsigned quads, unsigned groups) const {
+    const unsigned lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    if (g * 4 + wave < quads)
+      *reinterpret_cast<u32x4*>(out + (static_cast<size_t>(rb) * quads + g * 4 + wave) * 1024 + lane * 16) =
+          *reinterpret_cast<const u32x4*>(&codes[at(wave, lane >> 4, lane & 15, 0)]);
+    if (wave == 0)
+      *reinterpret_cast<unsigned*>(out_scales + (static_cast<size_t>(rb) * groups + g) * 256 + lane * 4) =
+          reinterpret_cast<const unsigned*>(scales)[lane];
+  }
 };
 
-// Blocks along a row. A wave takes four rows one after the other (their loads in flight together), 512
-// elements of each: 16 lanes a quad, eight elements a lane, so four lanes share a block.
+// Blocks along a row. A wave takes 512 elements of four rows, their loads in flight together.
 template <typename T>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const T* __restrict__ x, int64_t stride, unsigned rows,
                                                             int k, Div groups, unsigned quads, char* __restrict__ codes,
                                                             char* __restrict__ scales) {
   __shared__ Piece piece;
   const unsigned rb = groups.quot(blockIdx.x), g = blockIdx.x - rb * groups.d;
-  const unsigned lane = threadIdx.x & 63, wave = threadIdx.x >> 6, quad = lane >> 4, block = (lane >> 2) & 3;
+  const unsigned lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   unsigned w[4][8 / Elem<T>::kPerWord];
+  with_reach<T>(static_cast<int>(g * 512 + 512), k, [&](auto how) {
+#pragma unroll
+    for (unsigned i = 0; i < 4; ++i)
+      load8<decltype(how)::value>(x + static_cast<int64_t>(min(rb * 16 + wave * 4 + i, rows - 1)) * stride,
+                                  static_cast<int>(g * 512 + lane * 8), k, w[i]);
+  });
 #pragma unroll
   for (unsigned i = 0; i < 4; ++i) {
-    const unsigned row = rb * 16 + wave * 4 + i;
-    if (row < rows) load8(x + static_cast<int64_t>(row) * stride, static_cast<int>(g * 512 + lane * 8), k, w[i]);
-    else
+    if (rb * 16 + wave * 4 + i >= rows)
       for (unsigned& v : w[i]) v = 0;
-  }
-#pragma unroll
-  for (unsigned i = 0; i < 4; ++i) {
-    unsigned m = 0;
-#pragma unroll
-    for (unsigned v : w[i]) m = Elem<T>::amax(m, v);
-    m = Elem<T>::amax_f32(m);
-    m = max(m, dpp<kXor1>(m));
-    m = max(m, dpp<kXor2>(m));
-    const unsigned byte = scale_byte(m);
-    piece.codes[Piece::at(quad, block, wave * 4 + i, lane & 3)] = byte == 255 ? 0u : codes8<T>(w[i], scale_of(byte));
-    if ((lane & 3) == 0) piece.scales[(block * 16 + wave * 4 + i) * 4 + quad] = static_cast<unsigned char>(byte);
+    piece.template put<T>(w[i], wave * 4 + i, lane);
   }
   __syncthreads();
-  if (g * 4 + wave < quads)
-    *reinterpret_cast<u32x4*>(codes + (static_cast<size_t>(rb) * quads + g * 4 + wave) * 1024 + lane * 16) =
-        *reinterpret_cast<const u32x4*>(&piece.codes[Piece::at(wave, lane >> 4, lane & 15, 0)]);
-  if (wave == 0)
-    *reinterpret_cast<unsigned*>(scales + (static_cast<size_t>(rb) * groups.d + g) * 256 + lane * 4) =
-        reinterpret_cast<const unsigned*>(piece.scales)[lane];
+  piece.store(codes, scales, rb, g, quads, groups.d);
 }
 
 // Blocks down a column (the result's rows are x's columns), and with ROWS along the rows too, from one
-// reading. A workgroup takes 128 x 128 elements: as they arrive, 16 lanes on a row's quad, they are
-// quantised along the row and left in LDS; then wave b takes block b of every column, a lane two
-// columns of a 16-bit type (a word of each of 32 rows) or one and then another of f32.
+// reading. A workgroup takes 32 rows x 512 columns, whole KiB of a row of a 16-bit type at a time: as they
+// arrive they are quantised along the row, as above, and left in LDS; then each thread takes two columns,
+// neighbours in a 16-bit type (a word of each row), 256 apart in f32.
 template <typename T, bool ROWS>
 __global__ void __launch_bounds__(256) quantize_tile_kernel(const T* __restrict__ x, int64_t stride, unsigned rows,
-                                                            int k, Div tiles_k, char* __restrict__ row_codes,
+                                                            int k, Div groups, char* __restrict__ row_codes,
                                                             char* __restrict__ row_scales, char* __restrict__ col_codes,
                                                             char* __restrict__ col_scales) {
   constexpr int kWords = 8 / Elem<T>::kPerWord;  // of eight elements
-  constexpr int kRow = 16 * kWords;              // words of a row of the tile
-  __shared__ __attribute__((aligned(16))) unsigned tile[128 * kRow];
-  const unsigned tr = tiles_k.quot(blockIdx.x), tc = blockIdx.x - tr * tiles_k.d;
-  const unsigned lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, block = l >> 2;
-  const unsigned row_groups = (tiles_k.d + 3) / 4, quads = (rows + 127) / 128, col_groups = (quads + 3) / 4;
+  constexpr int kRow = 64 * kWords;              // words of a row of the tile
+  __shared__ __attribute__((aligned(16))) unsigned tile[32 * kRow];
+  __shared__ Piece piece[ROWS ? 2 : 1];
+  const unsigned tr = groups.quot(blockIdx.x), g = blockIdx.x - tr * groups.d;
+  const unsigned lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   unsigned w[8][kWords];
+  with_reach<T>(static_cast<int>(g * 512 + 512), k, [&](auto how) {
+#pragma unroll
+    for (unsigned i = 0; i < 8; ++i)
+      load8<decltype(how)::value>(x + static_cast<int64_t>(min(tr * 32 + wave * 8 + i, rows - 1)) * stride,
+                                  static_cast<int>(g * 512 + lane * 8), k, w[i]);
+  });
 #pragma unroll
   for (unsigned i = 0; i < 8; ++i) {
-    const unsigned row = tr * 128 + wave * 32 + i * 4 + (lane >> 4);
-    if (row < rows) load8(x + static_cast<int64_t>(row) * stride, static_cast<int>(tc * 128 + l * 8), k, w[i]);
-    else
+    const unsigned r = wave * 8 + i;
+    if (tr * 32 + r >= rows)
       for (unsigned& v : w[i]) v = 0;
-  }
-#pragma unroll
-  for (unsigned i = 0; i < 8; ++i) {
-    const unsigned r = wave * 32 + i * 4 + (lane >> 4), row = tr * 128 + r;
 #pragma unroll
     for (int p = 0; p < kWords; p += 4)
-      *reinterpret_cast<u32x4*>(&tile[r * kRow + l * kWords + p]) = u32x4{w[i][p], w[i][p + 1], w[i][p + 2], w[i][p + 3]};
-    if constexpr (ROWS) {
-      unsigned m = 0;
+      *reinterpret_cast<u32x4*>(&tile[r * kRow + lane * kWords + p]) = u32x4{w[i][p], w[i][p + 1], w[i][p + 2], w[i][p + 3]};
+    if constexpr (ROWS) piece[r >> 4].template put<T>(w[i], r & 15, lane);
+  }
+  __syncthreads();
+  if constexpr (ROWS) {
+    const unsigned quads = (static_cast<unsigned>(k) + 127) / 128;
 #pragma unroll
-      for (unsigned v : w[i]) m = Elem<T>::amax(m, v);
-      m = Elem<T>::amax_f32(m);
-      m = max(m, dpp<kXor1>(m));
-      m = max(m, dpp<kXor2>(m));
-      const unsigned byte = scale_byte(m);
-      const unsigned c = byte == 255 ? 0u : codes8<T>(w[i], scale_of(byte));
-      if ((row >> 4) < (rows + 15) >> 4) {
-        *reinterpret_cast<unsigned*>(row_codes + (static_cast<size_t>(row >> 4) * tiles_k.d + tc) * 1024 + block * 256 +
-                                     (row & 15) * 16 + (l & 3) * 4) = c;
-        if ((l & 3) == 0) {
-          char* s = row_scales + (static_cast<size_t>(row >> 4) * row_groups + (tc >> 2)) * 256 + block * 64 + (row & 15) * 4;
-          s[tc & 3] = static_cast<char>(byte);
-          if (tc + 1 == tiles_k.d)
-            for (unsigned j = (tc & 3) + 1; j < 4; ++j) s[j] = 0;
-        }
+    for (unsigned h = 0; h < 2; ++h)
+      if (tr * 2 + h < (rows + 15) / 16) piece[h].store(row_codes, row_scales, tr * 2 + h, g, quads, groups.d);
+  }
+  unsigned v[64 / Elem<T>::kPerWord];  // 32 elements of one column after 32 of the other
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    if constexpr (Elem<T>::kPerWord == 2) {
+      const unsigned a = tile[2 * i * kRow + threadIdx.x], b = tile[(2 * i + 1) * kRow + threadIdx.x];
+      v[i] = (a & 0xffffu) | (b << 16);
+      v[16 + i] = (a >> 16) | (b & 0xffff0000u);
+    } else {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        v[2 * i + h] = tile[(2 * i + h) * kRow + threadIdx.x];
+        v[32 + 2 * i + h] = tile[(2 * i + h) * kRow + 256 + threadIdx.x];
       }
     }
   }
-  __syncthreads();
-  auto store = [&](unsigned col, const unsigned* v) {  // 32 elements of a column
-    if (static_cast<int>(col) >= (k + 15) / 16 * 16) return;
+  // row tr of tiles is block tr % 4 of quad tr / 4 down the columns
+  const unsigned quads = (rows + 127) / 128, q = tr >> 2, b = tr & 3, col_groups = (quads + 3) / 4;
+#pragma unroll
+  for (unsigned h = 0; h < 2; ++h) {
+    const unsigned col = g * 512 + (Elem<T>::kPerWord == 2 ? threadIdx.x * 2 + h : h * 256 + threadIdx.x);
+    const unsigned* e = v + h * (32 / Elem<T>::kPerWord);
     unsigned m = 0;
 #pragma unroll
-    for (int i = 0; i < 32 / Elem<T>::kPerWord; ++i) m = Elem<T>::amax(m, v[i]);
+    for (int i = 0; i < 32 / Elem<T>::kPerWord; ++i) m = Elem<T>::amax(m, e[i]);
     const unsigned byte = scale_byte(Elem<T>::amax_f32(m));
     const float s = scale_of(byte);
     u32x4 o;
 #pragma unroll
-    for (int p = 0; p < 4; ++p) o[p] = byte == 255 ? 0u : codes8<T>(v + p * kWords, s);
-    *reinterpret_cast<u32x4*>(col_codes + (static_cast<size_t>(col >> 4) * quads + tr) * 1024 + wave * 256 + (col & 15) * 16) = o;
-    char* sp = col_scales + (static_cast<size_t>(col >> 4) * col_groups + (tr >> 2)) * 256 + wave * 64 + (col & 15) * 4;
-    sp[tr & 3] = static_cast<char>(byte);
-    if (tr + 1 == quads)
-      for (unsigned j = (tr & 3) + 1; j < 4; ++j) sp[j] = 0;
-  };
-  if constexpr (Elem<T>::kPerWord == 2) {
-    unsigned lo[16], hi[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const unsigned a = tile[(wave * 32 + 2 * i) * kRow + lane], b = tile[(wave * 32 + 2 * i + 1) * kRow + lane];
-      lo[i] = (a & 0xffffu) | (b << 16);
-      hi[i] = (a >> 16) | (b & 0xffff0000u);
-    }
-    store(tc * 128 + lane * 2, lo);
-    store(tc * 128 + lane * 2 + 1, hi);
-  } else {
-#pragma unroll 1
-    for (unsigned h = 0; h < 2; ++h) {
-      unsigned v[32];
-#pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] = tile[(wave * 32 + i) * kRow + h * 64 + lane];
-      store(tc * 128 + h * 64 + lane, v);
+    for (int p = 0; p < 4; ++p) o[p] = byte == 255 ? 0u : codes8<T>(e + p * kWords, s);
+    if (col < (static_cast<unsigned>(k) + 15) / 16 * 16) {
+      *reinterpret_cast<u32x4*>(col_codes + (static_cast<size_t>(col >> 4) * quads + q) * 1024 + b * 256 + (col & 15) * 16) = o;
+      char* sp = col_scales + (static_cast<size_t>(col >> 4) * col_groups + (q >> 2)) * 256 + b * 64 + (col & 15) * 4;
+      sp[q & 3] = static_cast<char>(byte);
+      if (q + 1 == quads)
+        for (unsigned j = (q & 3) + 1; j < 4; ++j) sp[j] = 0;
     }
   }
 }
@@ -205,9 +206,9 @@ unsigned blocks_for(int64_t n, int64_t per) { return static_cast<unsigned>((n + 
 template <typename T, bool ROWS>
 void launch_tiles(const T* x, int64_t rows, int64_t k, int64_t stride, char* row_codes, char* row_scales,
                   char* col_codes, char* col_scales, hipStream_t s) {
-  const unsigned tiles_k = static_cast<unsigned>(mx_quads(k));
-  hipLaunchKernelGGL((quantize_tile_kernel<T, ROWS>), dim3(tiles_k * static_cast<unsigned>(mx_quads(rows))), dim3(256), 0, s,
-                     x, stride, static_cast<unsigned>(rows), static_cast<int>(k), Div(tiles_k), row_codes, row_scales,
+  const unsigned groups = static_cast<unsigned>(mx_groups(k));
+  hipLaunchKernelGGL((quantize_tile_kernel<T, ROWS>), dim3(static_cast<unsigned>(mx_quads(rows) * 4) * groups), dim3(256), 0, s,
+                     x, stride, static_cast<unsigned>(rows), static_cast<int>(k), Div(groups), row_codes, row_scales,
                      col_codes, col_scales);
 }
 
