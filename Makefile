@@ -79,7 +79,7 @@ build/obj/hip/burn_dtypes.o: csrc/hip/burn_dtypes.hip $(HIP_HDR)
 	$(HIPCC) $(HIPFLAGS) $(BURN16_FLAGS) -c $< -o $@
 
 # MXFP4 operators: in the Python extension only, not in the probe plugin.
-MX_OBJ := build/obj/hip/mx_quant.o build/obj/hip/mx_product.o
+MX_OBJ := build/obj/hip/mx_quant.o build/obj/hip/mx_product.o build/obj/hip/mx_load.o
 $(MX_OBJ): build/obj/hip/%.o: csrc/hip/%.hip $(HIP_HDR)
 	@mkdir -p $(dir $@)
 	$(HIPCC) $(HIPFLAGS) -c $< -o $@

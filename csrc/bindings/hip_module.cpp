@@ -6,11 +6,28 @@
 
 #include "../hip/hip_api.h"
 #include "../hip/mx.h"
+#include "../hip/mx_load.h"
 
 namespace py = pybind11;
 using namespace gpumon_hip;
 
 static void* P(uintptr_t x) { return reinterpret_cast<void*>(x); }
+
+static py::dict load_stats(const LoadStats& s) {
+  py::dict d;
+  d["launches"] = s.launches;
+  d["busy_s"] = s.busy_s;
+  d["flops"] = s.flops;
+  d["bytes"] = s.bytes;
+  d["mfma_s"] = s.mfma_s;
+  d["hbm_s"] = s.hbm_s;
+  d["wall_s"] = s.wall_s;
+  d["tflops"] = s.mfma_s > 0 ? s.flops / s.mfma_s / 1e12 : 0.0;  // rate while MFMA batches ran
+  d["tbps"] = s.hbm_s > 0 ? s.bytes / s.hbm_s / 1e12 : 0.0;      // rate while HBM batches ran
+  d["tflops_wall"] = s.wall_s > 0 ? s.flops / s.wall_s / 1e12 : 0.0;  // averaged over wall time
+  d["tbps_wall"] = s.wall_s > 0 ? s.bytes / s.wall_s / 1e12 : 0.0;
+  return d;
+}
 
 PYBIND11_MODULE(_hip, m) {
   m.doc() = "gpumon gfx950 HIP kernels (probe ring buffer + synthetic MFMA/HBM load)";
@@ -71,7 +88,7 @@ PYBIND11_MODULE(_hip, m) {
   }, py::arg("dev"), py::arg("a_codes"), py::arg("a_scales"), py::arg("b_codes"), py::arg("b_scales"), py::arg("m"),
      py::arg("n"), py::arg("k"), py::arg("c"), py::arg("dtype"), py::arg("stride"), py::arg("workspace") = 0,
      py::arg("workspace_bytes") = 0, py::arg("stream") = 0);
-  m.def("mx_linear_workspace", &mx_linear_workspace, py::arg("m"), py::arg("n"), py::arg("k"));
+  m.def("mx_linear_workspace", &mx_linear_workspace, py::arg("m"), py::arg("n"), py::arg("k"), py::arg("dtype"));
   m.def("mx_linear", [](int dev, uintptr_t x, const std::string& dtype, int64_t x_stride, uintptr_t w_codes,
                         uintptr_t w_scales, int64_t m, int64_t n, int64_t k, uintptr_t y, int64_t y_stride,
                         uintptr_t workspace, size_t workspace_bytes, uintptr_t stream) {
@@ -103,21 +120,22 @@ PYBIND11_MODULE(_hip, m) {
       })
       .def_property_readonly("running", &LoadGen::running)
       .def("stats", [](LoadGen& g) {
-        LoadStats s = g.stats();
-        py::dict d;
-        d["launches"] = s.launches;
-        d["busy_s"] = s.busy_s;
-        d["flops"] = s.flops;
-        d["bytes"] = s.bytes;
-        d["mfma_s"] = s.mfma_s;
-        d["hbm_s"] = s.hbm_s;
-        d["wall_s"] = s.wall_s;
-        d["tflops"] = s.mfma_s > 0 ? s.flops / s.mfma_s / 1e12 : 0.0;  // rate while MFMA batches ran
-        d["tbps"] = s.hbm_s > 0 ? s.bytes / s.hbm_s / 1e12 : 0.0;      // rate while HBM batches ran
-        d["tflops_wall"] = s.wall_s > 0 ? s.flops / s.wall_s / 1e12 : 0.0;  // averaged over wall time
-        d["tbps_wall"] = s.wall_s > 0 ? s.bytes / s.wall_s / 1e12 : 0.0;
-        return d;
+        return load_stats(g.stats());
       });
+
+  py::class_<MxLoad>(m, "MxLoad")
+      .def(py::init<int, int64_t, int64_t, int64_t, double, double>(), py::arg("dev"), py::arg("rows") = 4096,
+           py::arg("n") = 8192, py::arg("k") = 8192, py::arg("duty") = 1.0, py::arg("period_s") = 0.0)
+      .def("start", [](MxLoad& g) {
+        py::gil_scoped_release nogil;
+        g.start();
+      })
+      .def("stop", [](MxLoad& g) {
+        py::gil_scoped_release nogil;
+        g.stop();
+      })
+      .def_property_readonly("running", &MxLoad::running)
+      .def("stats", [](MxLoad& g) { return load_stats(g.stats()); });
 
   py::class_<XgmiLoad>(m, "XgmiLoad")
       .def(py::init<int, int, size_t, std::string, int>(), py::arg("src"), py::arg("dst"),

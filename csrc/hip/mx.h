@@ -56,7 +56,7 @@ void launch_mx_product(int dev, const void* a_codes, const void* a_scales, const
                        int64_t m, int64_t n, int64_t k, void* c, const std::string& dtype, int64_t stride,
                        void* workspace, size_t workspace_bytes, void* stream);
 // y [m, n] = Q(x) w^T: x [m, k] in `dtype`, quantised here; y has the same type.
-size_t mx_linear_workspace(int64_t m, int64_t n, int64_t k);
+size_t mx_linear_workspace(int64_t m, int64_t n, int64_t k, const std::string& dtype);
 void launch_mx_linear(int dev, const void* x, const std::string& dtype, int64_t x_stride, const void* w_codes,
                       const void* w_scales, int64_t m, int64_t n, int64_t k, void* y, int64_t y_stride,
                       void* workspace, size_t workspace_bytes, void* stream);

@@ -530,10 +530,14 @@ void check_product(int64_t m, int64_t n, int64_t k, int64_t stride) {
 }
 
 // Whether a linear layer's rows are quantised by the workgroups that multiply them, each for itself, or
-// once by a launch before. The launch costs 2.6 us; on the way, 64 Ki elements a compute unit cost 2 us.
-bool quantise_on_the_way(int64_t m, int64_t n, int64_t k) {
-  const int64_t blocks = (n + 15) / 16, workgroups = m > 4 && blocks > kComputeUnits ? (blocks + 1) / 2 : blocks;
-  return m <= 8 && m * k * ((workgroups + kComputeUnits - 1) / kComputeUnits) <= (1 << 17);
+// once by a launch before. The launch costs 2.5 us; on the way, each workgroup reads and quantises all of
+// x: 400 KB of it a compute unit, over its workgroups one after the other, take about as long (bf16, 8
+// rows: 8192 x 8192 weights 10.4 us on the way, 12.6 with the launch; 4096 x 28672 19.6 and 18.5).
+bool quantise_on_the_way(int64_t m, int64_t n, int64_t k, int size) {
+  const int64_t blocks = (n + 15) / 16;
+  // row blocks in hand at once: two workgroups a compute unit for up to four rows, else one of one or two
+  const int64_t at_once = m > 4 && blocks <= kComputeUnits ? kComputeUnits : 2 * kComputeUnits;
+  return m <= 8 && m * k * size * ((blocks + at_once - 1) / at_once) <= 400000;
 }
 
 size_t round16(size_t b) { return (b + 15) / 16 * 16; }
@@ -609,9 +613,9 @@ void launch_mx_product(int dev, const void* a_codes, const void* a_scales, const
   check(hipGetLastError(), "mx_product");
 }
 
-size_t mx_linear_workspace(int64_t m, int64_t n, int64_t k) {
+size_t mx_linear_workspace(int64_t m, int64_t n, int64_t k, const std::string& dtype) {
   check_product(m, n, k, n);
-  if (quantise_on_the_way(m, n, k)) return 0;
+  if (quantise_on_the_way(m, n, k, size_of(type_of(dtype, "mx_linear: dtype must be bf16|f16|f32")))) return 0;
   return round16(static_cast<size_t>(mx_codes_bytes(m, k) + mx_scales_bytes(m, k))) + mx_product_workspace(m, n, k);
 }
 
@@ -625,7 +629,7 @@ void launch_mx_linear(int dev, const void* x, const std::string& dtype, int64_t 
   require(x && w_codes && w_scales && y, "mx_linear: null pointer");
   require(aligned(x, size_of(t)) && aligned(y, size_of(t)) && aligned(w_codes, 16) && aligned(w_scales, 16),
           "mx_linear: x and y aligned to their type, codes and scales to 16 bytes");
-  if (quantise_on_the_way(m, n, k)) {
+  if (quantise_on_the_way(m, n, k, size_of(t))) {
     OnDevice on(dev);
     auto s = static_cast<hipStream_t>(stream);
     with_type(t, [&](auto e) {
@@ -642,7 +646,7 @@ void launch_mx_linear(int dev, const void* x, const std::string& dtype, int64_t 
     check(hipGetLastError(), "mx_linear");
     return;
   }
-  require(workspace && workspace_bytes >= mx_linear_workspace(m, n, k), "mx_linear: workspace too small");
+  require(workspace && workspace_bytes >= mx_linear_workspace(m, n, k, dtype), "mx_linear: workspace too small");
   require(aligned(workspace, 16), "mx_linear: workspace aligned to 16 bytes");
   auto codes = static_cast<char*>(workspace);
   auto scales = codes + mx_codes_bytes(m, k);

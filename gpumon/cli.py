@@ -242,7 +242,7 @@ def cmd_load(args) -> int:
     from .ops.load import SyntheticLoad
 
     with SyntheticLoad(args.device, args.kind, duty=args.duty, mfma_dtype=args.dtype, period_s=args.period,
-                       pcie_direction=args.pcie_direction) as load:
+                       pcie_direction=args.pcie_direction, mx_rows=args.rows) as load:
         time.sleep(args.seconds)
         print(json.dumps(load.stats()))
     return 0
@@ -318,7 +318,8 @@ def build_parser() -> argparse.ArgumentParser:
     s.set_defaults(fn=cmd_probe)
     s = sub.add_parser("load", help="synthetic gfx950 load")
     s.add_argument("--device", type=int, default=0)
-    s.add_argument("--kind", choices=["mfma", "hbm", "mixed", "concurrent", "partial", "pcie"], default="mixed")
+    s.add_argument("--kind", choices=["mfma", "hbm", "mixed", "concurrent", "partial", "pcie", "mxlinear"],
+                   default="mixed")
     s.add_argument("--pcie-direction", choices=["h2d", "d2h", "both"], default="both",
                    help="--kind pcie: pinned host -> device, device -> host, or both at once")
     s.add_argument("--duty", type=float, default=1.0)
@@ -326,6 +327,9 @@ def build_parser() -> argparse.ArgumentParser:
     s.add_argument("--seconds", type=float, default=10.0)
     s.add_argument("--dtype", default="bf16", choices=["bf16", "f16", "fp8", "f32", "f64", "i8", "mxfp8", "mxfp4"],
                    help="matrix path of the mfma burn")
+    s.add_argument("--rows", type=int, default=4096,
+                   help="--kind mxlinear: rows a layer takes at once (1-64: decode, weights streamed from HBM; "
+                        "thousands: prompts, the 4-bit matrix path)")
     s.set_defaults(fn=cmd_load)
     s = sub.add_parser("doctor", help="check what this node gives the exporter (backend, sysfs, KFD, hostPID, "
                                       "kubelet / CRI sockets, RAS, rt_priority, on-device plugins)")

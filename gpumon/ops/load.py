@@ -18,6 +18,11 @@ launches of the gfx950 kernels in ``csrc/hip/kernels.hip``:
   ``d2h`` / ``both`` on two streams): the host link's known traffic, against which
   ``gpu_pcie_bandwidth_bytes_per_second`` is checked (native ``PcieLoad``; ``stats()`` gives
   ``h2d_bytes`` / ``d2h_bytes`` and ``GBps_wall``, no FLOPs).
+* ``mxlinear`` — MXFP4 linear layers on random data (``gpumon.ops.mx``, native ``MxLoad``): ``mx_rows``
+  rows of ``mx_k`` bf16 activations, quantised and multiplied with ``mx_n`` x ``mx_k`` quantised weights,
+  layer after layer. Many rows (prompts, the default) load the 4-bit matrix path with what a real
+  product moves; few (decode: 1-64) stream the weights from HBM. ``stats()["flops"]`` and
+  ``["bytes"]`` are both over the same GPU time.
 
 ``period_s`` > 0 turns ``duty`` into long bursts (``duty * period_s`` busy, then idle to the end
 of the period: a training step's compute / communication phases) instead of an idle gap after
@@ -32,7 +37,7 @@ from __future__ import annotations
 
 from .._native import hip
 
-KINDS = ("mfma", "hbm", "mixed", "concurrent", "partial", "pcie")
+KINDS = ("mfma", "hbm", "mixed", "concurrent", "partial", "pcie", "mxlinear")
 PCIE_DIRECTIONS = ("h2d", "d2h", "both")
 DTYPES = ("bf16", "f16", "fp8", "f32", "f64", "i8", "mxfp8", "mxfp4")
 
@@ -40,7 +45,8 @@ DTYPES = ("bf16", "f16", "fp8", "f32", "f64", "i8", "mxfp8", "mxfp4")
 class SyntheticLoad:
     def __init__(self, dev: int = 0, kind: str = "mixed", duty: float = 1.0, hbm_bytes: int = 1 << 30,
                  mfma_iters: int = 8192, mfma_shape: int = 16, mfma_dtype: str = "bf16", period_s: float = 0.0,
-                 pcie_direction: str = "both", pcie_bytes: int = 256 << 20):
+                 pcie_direction: str = "both", pcie_bytes: int = 256 << 20, mx_rows: int = 4096, mx_n: int = 8192,
+                 mx_k: int = 8192):
         if kind not in KINDS:
             raise ValueError(f"load kind {kind!r}: one of {', '.join(KINDS)}")
         if mfma_dtype not in DTYPES:
@@ -49,7 +55,11 @@ class SyntheticLoad:
             raise ValueError(f"duty {duty}: in (0, 1]")
         if mfma_shape not in (16, 32):
             raise ValueError(f"mfma_shape {mfma_shape}: 16 or 32")
-        if kind == "pcie":
+        if min(mx_rows, mx_n, mx_k) < 1:
+            raise ValueError(f"mx_rows, mx_n, mx_k {mx_rows}, {mx_n}, {mx_k}: at least 1")
+        if kind == "mxlinear":
+            self._g = hip().MxLoad(dev, mx_rows, mx_n, mx_k, duty, period_s)
+        elif kind == "pcie":
             if pcie_direction not in PCIE_DIRECTIONS:
                 raise ValueError(f"pcie_direction {pcie_direction!r}: one of {', '.join(PCIE_DIRECTIONS)}")
             self._g = hip().PcieLoad(dev, pcie_bytes, pcie_direction, duty)

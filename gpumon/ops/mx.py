@@ -216,7 +216,7 @@ def linear(x, w: MxTensor):
     y = torch.empty(*x.shape[:-1], n, dtype=x.dtype, device=x.device)
     if y.numel():
         h, dev = hip(), x.device.index
-        need = h.mx_linear_workspace(m, n, w.k)
+        need = h.mx_linear_workspace(m, n, w.k, DTYPES[x.dtype])
         ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
         h.mx_linear(dev, x2.data_ptr(), DTYPES[x.dtype], _row_stride(x2), w._codes, w._scales, m, n, w.k, y.data_ptr(),
                     n, ws.data_ptr() if need else 0, need, _stream(x.device))

@@ -90,7 +90,7 @@ def test_native_product_refuses(H, over, match):
 
 
 def test_native_linear_refuses_a_small_workspace(H):
-    need = H.mx_linear_workspace(300, 400, 500)
+    need = H.mx_linear_workspace(300, 400, 500, "bf16")
     assert need > 0
     with pytest.raises(ValueError, match="workspace"):
         H.mx_linear(0, P, "bf16", 500, P, P, 300, 400, 500, P, 400, P, need - 1)

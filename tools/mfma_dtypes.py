@@ -2,7 +2,7 @@
 """Per-operand-type MFMA burns vs the PMC MOPS counters (gpu_mfma_tflops{dtype}) on one MI355X.
 
 For each matrix path (bf16, f16, fp8, f32, f64, i8, and the block-scaled f8f6f4 path with fp8 and
-fp4 operands): the K2 load generator burns that path (its FLOPs timed with HIP events) while a
+fp4 operands; `mxlinear`: real MXFP4 linear layers): the K2 load generator burns that path (its FLOPs timed with HIP events) while a
 0.4 s device-counting window samples every MOPS counter. Prints one JSON line: per dtype the
 event-timed TFLOP/s, the TFLOP/s each MOPS counter reported, and MFMA busy. Fresh process, no torch
 (PMC registers before HIP; a second HIP runtime in the process would trip the profiler)."""
@@ -27,7 +27,9 @@ def main():
     res = {}
     for dt in sys.argv[1:] or ("bf16", "f16", "fp8", "mxfp8", "mxfp4", "i8", "f32", "f64"):
         # long launches (7-30 ms): the host sync between 4-launch batches stays < 0.5 % of the window
-        with SyntheticLoad(0, "mfma", mfma_dtype=dt, mfma_iters=16384) as load:
+        # mxlinear: MXFP4 linear layers instead of a burn (their quantisation is part of the event time)
+        with (SyntheticLoad(0, "mxlinear") if dt == "mxlinear"
+              else SyntheticLoad(0, "mfma", mfma_dtype=dt, mfma_iters=16384)) as load:
             time.sleep(1.0)
             s0 = load.stats()
             raw = P.sample(0, DEFAULT_COUNTERS, 0.4)
