@@ -98,6 +98,28 @@ PYBIND11_MODULE(_hip, m) {
      py::arg("m"), py::arg("n"), py::arg("k"), py::arg("y"), py::arg("y_stride"), py::arg("workspace") = 0,
      py::arg("workspace_bytes") = 0, py::arg("stream") = 0);
 
+  m.def("mx_linear_train_saved", &mx_linear_train_saved, py::arg("m"), py::arg("n"), py::arg("k"));
+  m.def("mx_linear_train_workspace", &mx_linear_train_workspace, py::arg("m"), py::arg("n"), py::arg("k"));
+  m.def("mx_linear_train", [](int dev, uintptr_t x, const std::string& dtype, int64_t x_stride, uintptr_t w,
+                              const std::string& w_dtype, int64_t w_stride, int64_t m, int64_t n, int64_t k,
+                              uintptr_t y, int64_t y_stride, uintptr_t saved, size_t saved_bytes, uintptr_t workspace,
+                              size_t workspace_bytes, uintptr_t stream) {
+    launch_mx_linear_train(dev, P(x), dtype, x_stride, P(w), w_dtype, w_stride, m, n, k, P(y), y_stride, P(saved),
+                           saved_bytes, P(workspace), workspace_bytes, P(stream));
+  }, py::arg("dev"), py::arg("x"), py::arg("dtype"), py::arg("x_stride"), py::arg("w"), py::arg("w_dtype"),
+     py::arg("w_stride"), py::arg("m"), py::arg("n"), py::arg("k"), py::arg("y"), py::arg("y_stride"),
+     py::arg("saved"), py::arg("saved_bytes"), py::arg("workspace"), py::arg("workspace_bytes"), py::arg("stream") = 0);
+  m.def("mx_linear_grad_workspace", &mx_linear_grad_workspace, py::arg("m"), py::arg("n"), py::arg("k"));
+  m.def("mx_linear_grad", [](int dev, uintptr_t dy, const std::string& dtype, int64_t dy_stride, uintptr_t saved,
+                             int64_t m, int64_t n, int64_t k, uintptr_t dx, int64_t dx_stride, uintptr_t dw,
+                             const std::string& w_dtype, int64_t dw_stride, uintptr_t workspace, size_t workspace_bytes,
+                             uintptr_t stream) {
+    launch_mx_linear_grad(dev, P(dy), dtype, dy_stride, P(saved), m, n, k, P(dx), dx_stride, P(dw), w_dtype, dw_stride,
+                          P(workspace), workspace_bytes, P(stream));
+  }, py::arg("dev"), py::arg("dy"), py::arg("dtype"), py::arg("dy_stride"), py::arg("saved"), py::arg("m"),
+     py::arg("n"), py::arg("k"), py::arg("dx"), py::arg("dx_stride"), py::arg("dw"), py::arg("w_dtype"),
+     py::arg("dw_stride"), py::arg("workspace"), py::arg("workspace_bytes"), py::arg("stream") = 0);
+
   py::class_<LoadGen>(m, "LoadGen")
       .def(py::init([](int dev, std::string kind, double duty, size_t hbm_bytes, int mfma_iters, int shape,
                        std::string dtype, double period_s) {

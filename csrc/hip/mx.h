@@ -61,4 +61,20 @@ void launch_mx_linear(int dev, const void* x, const std::string& dtype, int64_t 
                       const void* w_scales, int64_t m, int64_t n, int64_t k, void* y, int64_t y_stride,
                       void* workspace, size_t workspace_bytes, void* stream);
 
+
+// Training step of a linear layer. Forward: y [m, n] = Q(x) Q(w)^T from x [m, k] and w [n, k], with x and w
+// quantised down their columns too, into `saved`. Backward: dx [m, k] = Q(dy) Q0(w), dw [n, k] =
+// Q0(dy)^T Q0(x), Q0 in blocks down the columns; dx or dw may be null. y and dx have x's type, dw w's.
+size_t mx_linear_train_saved(int64_t m, int64_t n, int64_t k);
+size_t mx_linear_train_workspace(int64_t m, int64_t n, int64_t k);
+void launch_mx_linear_train(int dev, const void* x, const std::string& dtype, int64_t x_stride, const void* w,
+                            const std::string& w_dtype, int64_t w_stride, int64_t m, int64_t n, int64_t k, void* y,
+                            int64_t y_stride, void* saved, size_t saved_bytes, void* workspace, size_t workspace_bytes,
+                            void* stream);
+size_t mx_linear_grad_workspace(int64_t m, int64_t n, int64_t k);
+void launch_mx_linear_grad(int dev, const void* dy, const std::string& dtype, int64_t dy_stride, const void* saved,
+                           int64_t m, int64_t n, int64_t k, void* dx, int64_t dx_stride, void* dw,
+                           const std::string& w_dtype, int64_t dw_stride, void* workspace, size_t workspace_bytes,
+                           void* stream);
+
 }  // namespace gpumon_hip

@@ -173,6 +173,7 @@ constexpr int kXor1 = 0xB1, kXor2 = 0x4E;
 struct Div {
   unsigned d, m;
   int s;
+  Div() : d(1), m(0), s(0) {}
   explicit Div(unsigned div) : d(div), m(0), s(0) {
     int l = 0;
     while ((1ull << l) < div) ++l;
@@ -184,25 +185,30 @@ struct Div {
   }
 };
 
-// A matrix's tiles in the order in which workgroups take them: bands of H rows of tiles, down each column
-// of a band. Workgroups run on the eight XCDs in turn, and each XCD takes a run of neighbours in this
-// order, so that what neighbours share meets in one cache.
+// Which of `total` pieces of work this workgroup takes in round r; false if none is left for it.
+// Workgroups run on the eight XCDs in turn, and each XCD takes a run of neighbours, so that what
+// neighbours share meets in one cache.
+__device__ __forceinline__ bool turn(unsigned total, unsigned r, unsigned& piece) {
+  const unsigned first = r * gridDim.x, place = blockIdx.x / 8;
+  const unsigned count = first < total ? min(total - first, gridDim.x) : 0, per = (count + 7) / 8;
+  const unsigned p = blockIdx.x % 8 * per + place;
+  piece = first + p;
+  return place < per && p < count;
+}
+
+// A matrix's tiles in the order in which they are taken: bands of H rows of tiles, down each column of a
+// band.
 template <unsigned H>
 struct Tiles {
   unsigned rows, cols, total;
   Div band, last;  // tiles of a band; rows of the last band
   Tiles(unsigned r, unsigned c) : rows(r), cols(c), total(r * c), band(H * c), last((r + H - 1) % H + 1) {}
-  unsigned whole_grid() const { return (total + 7) / 8 * 8; }
-  // tile `r` of this workgroup; false if it has none
-  __device__ __forceinline__ bool get(unsigned r, unsigned& row, unsigned& col) const {
-    const unsigned first = r * gridDim.x, place = blockIdx.x / 8;
-    const unsigned count = first < total ? min(total - first, gridDim.x) : 0, per = (count + 7) / 8;
-    const unsigned p = blockIdx.x % 8 * per + place, b = band.quot(first + p), in = first + p - b * band.d;
+  __device__ __forceinline__ void at(unsigned piece, unsigned& row, unsigned& col) const {
+    const unsigned b = band.quot(piece), in = piece - b * band.d;
     const bool whole = b * H + H <= rows;
     col = whole ? in / H : last.quot(in);
     row = b * H + in - col * (whole ? H : last.d);
     row = __builtin_amdgcn_readfirstlane(row), col = __builtin_amdgcn_readfirstlane(col);
-    return place < per && p < count;
   }
 };
 
@@ -242,6 +248,40 @@ void with_type(Type t, F f) {  // f(T{})
   else if (t == Type::f16) f(_Float16{});
   else f(float{});
 }
+
+// A quantised operand; and one in a buffer, codes then scales.
+struct Operand {
+  const char *codes, *scales;
+};
+inline Operand operand(const void* codes, const void* scales) {
+  return {static_cast<const char*>(codes), static_cast<const char*>(scales)};
+}
+inline size_t mx_bytes(int64_t rows, int64_t k) {  // a multiple of 256
+  return static_cast<size_t>(mx_codes_bytes(rows, k) + mx_scales_bytes(rows, k));
+}
+struct Quantized {
+  char* at;
+  int64_t rows, k;
+  char* scales() const { return at + mx_codes_bytes(rows, k); }
+  Operand operand() const { return {at, scales()}; }
+};
+
+// A matrix to quantise both ways: x [rows, k], its results in buffers as above.
+struct Source {
+  const void* x;
+  int64_t stride, rows, k;
+  char *along, *down;
+};
+void check_source(const Source& s, Type t);
+void launch_quantize_both(int dev, const Source* sources, int count, Type t, hipStream_t s);  // up to two
+
+// A product c [m, n] = a [m, k] b [n, k]^T.
+struct Job {
+  Operand a, b;
+  int64_t m, n, k;
+  void* c;
+  int64_t stride;
+};
 
 }  // namespace mx
 }  // namespace gpumon_hip

@@ -77,13 +77,22 @@ __device__ __forceinline__ void hold() {
 // a stage's operands are read into registers while the one before multiplies, so that the matrix
 // instructions wait for nothing but the barrier (Order). b's rows take the instruction's A side: a lane's four
 // sums are neighbours in a row of c.
+// One launch takes up to two products, the second's tiles after the first's.
 // SPLIT: the tiles' columns are taken `parts` times, each time with `per` of k's groups of quads, and each
 // part's sums go to a matrix of its own.
+struct Product {
+  const char *ac, *as, *bc, *bs;
+  void* c;
+  int64_t stride;
+  unsigned m, n, quads, per;
+  Div part_cols;
+  Tiles<8> tiles;
+};
+struct Products {
+  Product p[2];
+};
 template <typename T, int FM, int FN, int WM, int WN, int RESIDENT, bool SPLIT = false>
-__global__ void __launch_bounds__(64 * WM * WN, RESIDENT * WM * WN / 4)
-    product_tile_kernel(const char* __restrict__ ac, const char* __restrict__ as, const char* __restrict__ bc,
-                        const char* __restrict__ bs, unsigned m, unsigned n, unsigned quads, T* __restrict__ c,
-                        int64_t stride, Tiles<8> tiles, Div part_cols, unsigned per) {
+__global__ void __launch_bounds__(64 * WM * WN, RESIDENT * WM * WN / 4) product_tile_kernel(Products products) {
   constexpr int TM = FM * WM, TN = FN * WN, kChunks = TM + TN, kLoads = kChunks / (WM * WN);
   constexpr int kScaleLoads = kChunks >= 4 * WM * WN ? kChunks / (4 * WM * WN) : 1;
   constexpr int kStage = kChunks * 1024, kScales = kChunks * 256;
@@ -92,7 +101,6 @@ __global__ void __launch_bounds__(64 * WM * WN, RESIDENT * WM * WN / 4)
   constexpr int kParts = kPiece * static_cast<int>(sizeof(T)), kOut = 256 * kParts;
   __shared__ __attribute__((aligned(16))) char lds[4 * kStage + 2 * kScales + WM * WN * kOut];
   const unsigned lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const unsigned rbm = (m + 15) / 16, rbn = (n + 15) / 16, all_groups = (quads + 3) / 4;
   const unsigned wm = wave % WM, wn = wave / WM;
 
   Buffer src[kLoads], ssrc[kScaleLoads];
@@ -100,12 +108,13 @@ __global__ void __launch_bounds__(64 * WM * WN, RESIDENT * WM * WN / 4)
   // Where the loads come from: chunk x of a tile, a's TM first. Row blocks past the end read the last one
   // instead, and what comes of them is not stored. Past the last tile, and past the last quad, zeros come
   // without a read: four steps at a time are taken, and scales there are zeros too.
-  auto aim = [&](bool any, unsigned tm, unsigned tn) {
+  auto aim = [&](bool any, const Product& p, unsigned tm, unsigned tn) {
+    const unsigned rbm = (p.m + 15) / 16, rbn = (p.n + 15) / 16, quads = p.quads, all_groups = (quads + 3) / 4;
     unsigned g0 = 0;
     if constexpr (SPLIT) {
-      const unsigned part = part_cols.quot(tn);
-      tn -= part * part_cols.d;
-      g0 = part * per;
+      const unsigned part = p.part_cols.quot(tn);
+      tn -= part * p.part_cols.d;
+      g0 = part * p.per;
     }
     auto row_block = [&](unsigned x) {
       return x < TM ? min(tm * TM + x, rbm - 1) : min(tn * TN + x - TM, rbn - 1);
@@ -113,13 +122,13 @@ __global__ void __launch_bounds__(64 * WM * WN, RESIDENT * WM * WN / 4)
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       const unsigned x = wave * kLoads + i;
-      src[i] = buffer((x < TM ? ac : bc) + (static_cast<size_t>(row_block(x)) * quads + g0 * 4) * 1024,
+      src[i] = buffer((x < TM ? p.ac : p.bc) + (static_cast<size_t>(row_block(x)) * quads + g0 * 4) * 1024,
                       any ? (quads - g0 * 4) * 1024 : 0);
     }
 #pragma unroll
     for (int i = 0; i < kScaleLoads; ++i) {
       const unsigned x = (wave * kScaleLoads + i) * 4 % kChunks, first = row_block(x);
-      ssrc[i] = buffer((x < TM ? as : bs) + (static_cast<size_t>(first) * all_groups + g0) * 256,
+      ssrc[i] = buffer((x < TM ? p.as : p.bs) + (static_cast<size_t>(first) * all_groups + g0) * 256,
                        any ? ((row_block(x + 3) - first + 1) * all_groups - g0) * 256 : 0);
       soff[i] = (row_block(x + (lane >> 4)) - first) * all_groups * 256 + (lane & 15) * 16;
     }
@@ -152,9 +161,18 @@ __global__ void __launch_bounds__(64 * WM * WN, RESIDENT * WM * WN / 4)
     for (int j = 0; j < FN; ++j) sb[j] = *reinterpret_cast<const unsigned*>(p + (TM + wn * FN + j) * 256);
   };
 
-  unsigned tm = 0, tn = 0, round = 0;
-  if (!tiles.get(0, tm, tn)) return;
-  aim(true, tm, tn);
+  // the tile of round r: which product's, and where
+  auto tile_of = [&](unsigned r, unsigned& which, unsigned& row, unsigned& col) {
+    unsigned piece;
+    const unsigned first = products.p[0].tiles.total;
+    const bool any = turn(first + products.p[1].tiles.total, r, piece);
+    which = piece < first || !any ? 0 : 1;
+    products.p[which].tiles.at(piece - (which ? first : 0), row, col);
+    return any;
+  };
+  unsigned which = 0, tm = 0, tn = 0, round = 0;
+  if (!tile_of(0, which, tm, tn)) return;
+  aim(true, products.p[which], tm, tn);
   load_scales(0, 0);
 #pragma unroll
   for (int t = 0; t < 4; ++t)
@@ -214,19 +232,18 @@ __global__ void __launch_bounds__(64 * WM * WN, RESIDENT * WM * WN / 4)
     for (int i = 0; i < FM; ++i)
 #pragma unroll
       for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
-    unsigned next_m = 0, next_n = 0;
-    const bool more = tiles.get(round + 1, next_m, next_n);
-    unsigned groups = all_groups, col = tn;
-    T* part_c = c;
+    unsigned next = 0, next_m = 0, next_n = 0;
+    const bool more = tile_of(round + 1, next, next_m, next_n);
+    const Product& p = products.p[which];
+    unsigned groups = (p.quads + 3) / 4, col = tn, part = 0;
     if constexpr (SPLIT) {
-      const unsigned part = part_cols.quot(tn);
-      col -= part * part_cols.d;
-      groups = min(per, all_groups - part * per);
-      part_c += static_cast<size_t>(part) * m * n;
+      part = p.part_cols.quot(tn);
+      col -= part * p.part_cols.d;
+      groups = min(p.per, groups - part * p.per);
     }
 #pragma unroll 1
     for (unsigned g = 0; g < groups; ++g) {
-      if (g + 1 == groups) aim(more, next_m, next_n);
+      if (g + 1 == groups) aim(more, products.p[next], next_m, next_n);
       body(g, groups, Int<0>{});
       body(g, groups, Int<1>{});
       body(g, groups, Int<2>{});
@@ -236,7 +253,9 @@ __global__ void __launch_bounds__(64 * WM * WN, RESIDENT * WM * WN / 4)
     unsigned l = lane;
     asm volatile("" : "+v"(l));  // what follows from the lane is computed here, not kept through the loop above
     const unsigned row0 = (tm * WM + wm) * FM * 16, col0 = (col * WN + wn) * FN * 16, r = l & 15, q = l >> 4;
-    T* out = part_c + static_cast<int64_t>(row0) * stride + col0;
+    const unsigned m = p.m, n = p.n;
+    const int64_t stride = p.stride;
+    T* out = static_cast<T*>(p.c) + static_cast<size_t>(part) * m * n + static_cast<int64_t>(row0) * stride + col0;
     char* piece = lds + 4 * kStage + 2 * kScales + wave * kOut;
     auto leave = [&](auto store) {
 #pragma unroll
@@ -278,7 +297,7 @@ __global__ void __launch_bounds__(64 * WM * WN, RESIDENT * WM * WN / 4)
       });
     }
     if (!more) break;
-    tm = next_m, tn = next_n, ++round;
+    which = next, tm = next_m, tn = next_n, ++round;
   }
   __builtin_amdgcn_s_waitcnt(wait_imm(0, true));  // no load may arrive after the workgroup's memory is given back
 }
@@ -472,12 +491,12 @@ __global__ void __launch_bounds__(64 * kWaves) product_few_rows_kernel(Source so
 }
 
 template <typename T, int FM, int R, int U, typename Source>
-void few_rows(Source source, const void* bc, const void* bs, int64_t m, int64_t n, int64_t k, T* c, int64_t stride,
+void few_rows(Source source, const Operand& b, int64_t m, int64_t n, int64_t k, T* c, int64_t stride,
               hipStream_t s) {
   auto run = [&](auto kernel, int waves) {
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>((n + 16 * R - 1) / (16 * R))), dim3(64 * waves), 0, s, source,
-                       static_cast<const char*>(bc), static_cast<const char*>(bs), static_cast<unsigned>(m),
-                       static_cast<unsigned>(n), static_cast<unsigned>(mx_quads(k)), c, stride);
+                       b.codes, b.scales, static_cast<unsigned>(m), static_cast<unsigned>(n),
+                       static_cast<unsigned>(mx_quads(k)), c, stride);
   };
   // no more waves than groups of quads
   if (mx_groups(k) <= 4) run(product_few_rows_kernel<T, Source, FM, R, 1, 4>, 4);
@@ -505,21 +524,34 @@ struct Plan {
   enum Shape { kFew, k256, k128, k64x128, k64 } shape;
   unsigned parts, per;  // of k, and groups of quads a part
 };
-Plan plan(int64_t m, int64_t n, int64_t k) {
-  const int64_t groups = mx_groups(k);
-  const auto whole = static_cast<unsigned>(groups);
-  auto tiles = [&](int64_t tm, int64_t tn) { return (m + tm - 1) / tm * ((n + tn - 1) / tn); };
-  if (m <= 32 || (m <= kFewRows && tiles(64, 64) < 192)) return {Plan::kFew, 1, whole};
+// The largest tiles of which there are enough, over all of a launch's products; false if there are too few
+// of any.
+bool plan_tiles(const Job* jobs, int count, Plan& p) {
+  auto tiles = [&](int64_t tm, int64_t tn) {
+    int64_t t = 0;
+    for (int i = 0; i < count; ++i) t += (jobs[i].m + tm - 1) / tm * ((jobs[i].n + tn - 1) / tn);
+    return t;
+  };
+  bool deep = true, wide = true;
+  for (int i = 0; i < count; ++i) deep &= jobs[i].k > 512, wide &= jobs[i].n > 64;
   const int64_t big = tiles(256, 256);
-  if (big * 5 >= (big + kComputeUnits - 1) / kComputeUnits * kComputeUnits * 4 && groups > 1) return {Plan::k256, 1, whole};
-  if (tiles(128, 128) >= kEnough) return {Plan::k128, 1, whole};
-  if (n > 64 && tiles(64, 128) >= kEnough) return {Plan::k64x128, 1, whole};
-  const int64_t small = tiles(64, 64);
-  if (small * 2 <= kComputeUnits && groups >= 16) {
+  p.parts = 1;
+  if (deep && big * 5 >= (big + kComputeUnits - 1) / kComputeUnits * kComputeUnits * 4) p.shape = Plan::k256;
+  else if (tiles(128, 128) >= kEnough) p.shape = Plan::k128;
+  else if (wide && tiles(64, 128) >= kEnough) p.shape = Plan::k64x128;
+  else return p.shape = Plan::k64, false;
+  return true;
+}
+Plan plan(const Job& j) {
+  const int64_t groups = mx_groups(j.k), small = (j.m + 63) / 64 * ((j.n + 63) / 64);
+  Plan p{Plan::kFew, 1, static_cast<unsigned>(groups)};
+  if (j.m <= 32 || (j.m <= kFewRows && small < 192)) return p;
+  if (!plan_tiles(&j, 1, p) && small * 2 <= kComputeUnits && groups >= 16) {
     const int64_t parts = std::min<int64_t>(kComputeUnits / small, groups / 4), per = (groups + parts - 1) / parts;
-    return {Plan::k64, static_cast<unsigned>((groups + per - 1) / per), static_cast<unsigned>(per)};
+    p.parts = static_cast<unsigned>((groups + per - 1) / per);
+    p.per = static_cast<unsigned>(per);
   }
-  return {Plan::k64, 1, whole};
+  return p;
 }
 
 void check_product(int64_t m, int64_t n, int64_t k, int64_t stride) {
@@ -540,83 +572,140 @@ bool quantise_on_the_way(int64_t m, int64_t n, int64_t k, int size) {
   return m <= 8 && m * k * size * ((blocks + at_once - 1) / at_once) <= 400000;
 }
 
-size_t round16(size_t b) { return (b + 15) / 16 * 16; }
-
 }  // namespace
 }  // namespace mx
 
 using namespace mx;
 
+namespace mx {
+namespace {
+
+size_t job_workspace(const Job& j) {
+  const Plan p = plan(j);
+  return p.parts > 1 ? static_cast<size_t>(p.parts) * j.m * j.n * 4 : 0;
+}
+
+void check_job(const Job& j, Type t) {
+  check_product(j.m, j.n, j.k, j.stride);
+  if (j.m == 0 || j.n == 0) return;
+  require(j.a.codes && j.a.scales && j.b.codes && j.b.scales && j.c, "mx_product: null pointer");
+  require(aligned(j.a.codes, 16) && aligned(j.b.codes, 16) && aligned(j.a.scales, 16) && aligned(j.b.scales, 16) &&
+              aligned(j.c, size_of(t)),
+          "mx_product: codes and scales aligned to 16 bytes, the result to its type");
+}
+
+template <typename T, int FM, int FN, int WM, int WN, int RESIDENT, bool SPLIT = false>
+void run_tiles(int dev, const Job* jobs, int count, const Plan& plan, hipStream_t s) {
+  auto product = [&](const Job& j, bool any) {
+    const unsigned rows = static_cast<unsigned>((j.m + 16 * FM * WM - 1) / (16 * FM * WM));
+    const unsigned cols = static_cast<unsigned>((j.n + 16 * FN * WN - 1) / (16 * FN * WN));
+    Tiles<8> tiles(rows, cols * plan.parts);
+    if (!any) tiles.total = 0;
+    return Product{j.a.codes, j.a.scales, j.b.codes, j.b.scales, j.c, j.stride, static_cast<unsigned>(j.m),
+                   static_cast<unsigned>(j.n), static_cast<unsigned>(mx_quads(j.k)), plan.per, Div(cols), tiles};
+  };
+  const Products products{{product(jobs[0], true), product(jobs[count - 1], count > 1)}};
+  const unsigned total = products.p[0].tiles.total + products.p[1].tiles.total;
+  const unsigned grid = std::min((total + 7) / 8 * 8, static_cast<unsigned>(compute_units(dev) * RESIDENT));
+  hipLaunchKernelGGL((product_tile_kernel<T, FM, FN, WM, WN, RESIDENT, SPLIT>), dim3(grid), dim3(64 * WM * WN), 0, s,
+                     products);
+}
+
+// One product, or two in one launch.
+void run_jobs(int dev, Job* jobs, int count, const Plan& p, Type t, void* workspace, hipStream_t s) {
+  with_type(t, [&](auto e) {
+    using T = decltype(e);
+    Job& j = jobs[0];
+    switch (p.shape) {
+      case Plan::kFew: {
+        const QuantizedRows x{j.a.codes, j.a.scales, static_cast<unsigned>(mx_quads(j.k)),
+                              static_cast<unsigned>(mx_groups(j.k)), static_cast<unsigned>(mx_row_blocks(j.m))};
+        auto out = static_cast<T*>(j.c);
+        const bool narrow = j.n <= 16 * kComputeUnits;  // a row block a workgroup fills the chip better than two
+        if (j.m <= 16) few_rows<T, 1, 1, 2>(x, j.b, j.m, j.n, j.k, out, j.stride, s);
+        else if (j.m <= 32 && narrow) few_rows<T, 2, 1, 2>(x, j.b, j.m, j.n, j.k, out, j.stride, s);
+        else if (j.m <= 32) few_rows<T, 2, 2, 2>(x, j.b, j.m, j.n, j.k, out, j.stride, s);
+        else if (narrow) few_rows<T, 4, 1, 1>(x, j.b, j.m, j.n, j.k, out, j.stride, s);
+        else few_rows<T, 4, 2, 2>(x, j.b, j.m, j.n, j.k, out, j.stride, s);
+        break;
+      }
+      case Plan::k256: run_tiles<T, 8, 4, 2, 4, 1>(dev, jobs, count, p, s); break;
+      case Plan::k128: run_tiles<T, 4, 4, 2, 2, 2>(dev, jobs, count, p, s); break;
+      case Plan::k64x128: run_tiles<T, 2, 4, 2, 2, 2>(dev, jobs, count, p, s); break;
+      case Plan::k64:
+        if (p.parts == 1) {
+          run_tiles<T, 2, 2, 2, 2, 3>(dev, jobs, count, p, s);
+        } else {
+          auto out = static_cast<T*>(j.c);
+          const int64_t stride = j.stride;
+          j.c = workspace, j.stride = j.n;
+          run_tiles<float, 2, 2, 2, 2, 3, true>(dev, jobs, 1, p, s);
+          const unsigned quarters = static_cast<unsigned>((j.n + 3) / 4);
+          hipLaunchKernelGGL(product_sum_kernel<T>, dim3(static_cast<unsigned>((j.m * quarters + 255) / 256)), dim3(256), 0,
+                             s, static_cast<const float*>(workspace), p.parts, static_cast<unsigned>(j.m),
+                             static_cast<unsigned>(j.n), out, stride, Div(quarters));
+        }
+        break;
+    }
+  });
+}
+
+}  // namespace
+
+// Up to two products of one result type; together where each would take whole tiles by itself, so that
+// the chip is filled once, else one after the other with the workspace in common.
+size_t products_workspace(const Job* jobs, int count) {
+  size_t need = 0;
+  for (int i = 0; i < count; ++i) need = std::max(need, job_workspace(jobs[i]));
+  return need;
+}
+void launch_products(int dev, const Job* jobs, int count, Type t, void* workspace, size_t workspace_bytes, hipStream_t s) {
+  Job todo[2];
+  int n = 0;
+  for (int i = 0; i < count; ++i) {
+    check_job(jobs[i], t);
+    if (jobs[i].m && jobs[i].n) todo[n++] = jobs[i];
+  }
+  if (n == 0) return;
+  const size_t need = products_workspace(todo, n);
+  require(need == 0 || (workspace && workspace_bytes >= need && aligned(workspace, 16)),
+          "mx_product: needs a workspace of mx_product_workspace bytes, aligned to 16");
+  OnDevice on(dev);
+  Plan p = plan(todo[0]);
+  if (n == 2) {
+    const Plan q = plan(todo[1]);
+    if (p.shape != Plan::kFew && q.shape != Plan::kFew && p.parts == 1 && q.parts == 1) {
+      plan_tiles(todo, 2, p);
+    } else {
+      run_jobs(dev, todo, 1, p, t, workspace, s);
+      todo[0] = todo[1];
+      p = q;
+      n = 1;
+    }
+  }
+  run_jobs(dev, todo, n, p, t, workspace, s);
+  check(hipGetLastError(), "mx_product");
+}
+
+}  // namespace mx
+
 size_t mx_product_workspace(int64_t m, int64_t n, int64_t k) {
   check_product(m, n, k, n);
-  const Plan p = plan(m, n, k);
-  return p.parts > 1 ? static_cast<size_t>(p.parts) * m * n * 4 : 0;
+  return job_workspace(Job{{}, {}, m, n, k, nullptr, n});
 }
 
 void launch_mx_product(int dev, const void* a_codes, const void* a_scales, const void* b_codes, const void* b_scales,
                        int64_t m, int64_t n, int64_t k, void* c, const std::string& dtype, int64_t stride,
                        void* workspace, size_t workspace_bytes, void* stream) {
   const Type t = type_of(dtype, "mx_product: dtype must be bf16|f16|f32");
-  check_product(m, n, k, stride);
-  if (m == 0 || n == 0) return;
-  require(a_codes && a_scales && b_codes && b_scales && c, "mx_product: null pointer");
-  require(aligned(a_codes, 16) && aligned(b_codes, 16) && aligned(a_scales, 16) && aligned(b_scales, 16) &&
-              aligned(c, size_of(t)),
-          "mx_product: codes and scales aligned to 16 bytes, the result to its type");
-  const size_t need = mx_product_workspace(m, n, k);
-  require(need == 0 || (workspace && workspace_bytes >= need && aligned(workspace, 16)),
-          "mx_product: needs a workspace of mx_product_workspace bytes, aligned to 16");
-  OnDevice on(dev);
-  auto s = static_cast<hipStream_t>(stream);
-  const Plan p = plan(m, n, k);
-  const auto um = static_cast<unsigned>(m), un = static_cast<unsigned>(n);
-  with_type(t, [&](auto e) {
-    using T = decltype(e);
-    auto out = static_cast<T*>(c);
-    auto run = [&](auto kernel, auto* to, int64_t to_stride, int tile_m, int tile_n, int waves, int resident) {
-      const unsigned cols = (un + tile_n - 1) / tile_n, rows = (um + tile_m - 1) / tile_m, total = rows * cols * p.parts;
-      const unsigned grid = std::min((total + 7) / 8 * 8, static_cast<unsigned>(compute_units(dev) * resident));
-      hipLaunchKernelGGL(kernel, dim3(grid), dim3(64 * waves), 0, s, static_cast<const char*>(a_codes),
-                         static_cast<const char*>(a_scales), static_cast<const char*>(b_codes),
-                         static_cast<const char*>(b_scales), um, un, static_cast<unsigned>(mx_quads(k)), to, to_stride,
-                         Tiles<8>(rows, cols * p.parts), Div(cols), p.per);
-    };
-    switch (p.shape) {
-      case Plan::kFew: {
-        const QuantizedRows x{static_cast<const char*>(a_codes), static_cast<const char*>(a_scales),
-                              static_cast<unsigned>(mx_quads(k)), static_cast<unsigned>(mx_groups(k)),
-                              static_cast<unsigned>(mx_row_blocks(m))};
-        const bool narrow = n <= 16 * kComputeUnits;  // a row block a workgroup fills the chip better than two
-        if (m <= 16) few_rows<T, 1, 1, 2>(x, b_codes, b_scales, m, n, k, out, stride, s);
-        else if (m <= 32 && narrow) few_rows<T, 2, 1, 2>(x, b_codes, b_scales, m, n, k, out, stride, s);
-        else if (m <= 32) few_rows<T, 2, 2, 2>(x, b_codes, b_scales, m, n, k, out, stride, s);
-        else if (narrow) few_rows<T, 4, 1, 1>(x, b_codes, b_scales, m, n, k, out, stride, s);
-        else few_rows<T, 4, 2, 2>(x, b_codes, b_scales, m, n, k, out, stride, s);
-        break;
-      }
-      case Plan::k256: run(product_tile_kernel<T, 8, 4, 2, 4, 1>, out, stride, 256, 256, 8, 1); break;
-      case Plan::k128: run(product_tile_kernel<T, 4, 4, 2, 2, 2>, out, stride, 128, 128, 4, 2); break;
-      case Plan::k64x128: run(product_tile_kernel<T, 2, 4, 2, 2, 2>, out, stride, 64, 128, 4, 2); break;
-      case Plan::k64:
-        if (p.parts == 1) {
-          run(product_tile_kernel<T, 2, 2, 2, 2, 3>, out, stride, 64, 64, 4, 3);
-        } else {
-          auto sums = static_cast<float*>(workspace);
-          run(product_tile_kernel<float, 2, 2, 2, 2, 3, true>, sums, n, 64, 64, 4, 3);
-          const unsigned quarters = (un + 3) / 4;
-          hipLaunchKernelGGL(product_sum_kernel<T>, dim3(static_cast<unsigned>((m * quarters + 255) / 256)), dim3(256), 0, s,
-                             sums, p.parts, um, un, out, stride, Div(quarters));
-        }
-        break;
-    }
-  });
-  check(hipGetLastError(), "mx_product");
+  const Job j{operand(a_codes, a_scales), operand(b_codes, b_scales), m, n, k, c, stride};
+  launch_products(dev, &j, 1, t, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
 }
 
 size_t mx_linear_workspace(int64_t m, int64_t n, int64_t k, const std::string& dtype) {
   check_product(m, n, k, n);
   if (quantise_on_the_way(m, n, k, size_of(type_of(dtype, "mx_linear: dtype must be bf16|f16|f32")))) return 0;
-  return round16(static_cast<size_t>(mx_codes_bytes(m, k) + mx_scales_bytes(m, k))) + mx_product_workspace(m, n, k);
+  return mx_bytes(m, k) + mx_product_workspace(m, n, k);
 }
 
 void launch_mx_linear(int dev, const void* x, const std::string& dtype, int64_t x_stride, const void* w_codes,
@@ -632,16 +721,17 @@ void launch_mx_linear(int dev, const void* x, const std::string& dtype, int64_t 
   if (quantise_on_the_way(m, n, k, size_of(t))) {
     OnDevice on(dev);
     auto s = static_cast<hipStream_t>(stream);
+    const Operand w = operand(w_codes, w_scales);
     with_type(t, [&](auto e) {
       using T = decltype(e);
       auto px = static_cast<const T*>(x);
       auto out = static_cast<T*>(y);
       const auto rows = static_cast<unsigned>(m);
       const int len = static_cast<int>(k);
-      if (m == 1) few_rows<T, 1, 1, 2>(PlainRows<T, 1>{px, x_stride, rows, len}, w_codes, w_scales, m, n, k, out, y_stride, s);
-      else if (m <= 4) few_rows<T, 1, 1, 2>(PlainRows<T, 4>{px, x_stride, rows, len}, w_codes, w_scales, m, n, k, out, y_stride, s);
-      else if (n <= 16 * kComputeUnits) few_rows<T, 1, 1, 1>(PlainRows<T, 8>{px, x_stride, rows, len}, w_codes, w_scales, m, n, k, out, y_stride, s);
-      else few_rows<T, 1, 2, 1>(PlainRows<T, 8>{px, x_stride, rows, len}, w_codes, w_scales, m, n, k, out, y_stride, s);
+      if (m == 1) few_rows<T, 1, 1, 2>(PlainRows<T, 1>{px, x_stride, rows, len}, w, m, n, k, out, y_stride, s);
+      else if (m <= 4) few_rows<T, 1, 1, 2>(PlainRows<T, 4>{px, x_stride, rows, len}, w, m, n, k, out, y_stride, s);
+      else if (n <= 16 * kComputeUnits) few_rows<T, 1, 1, 1>(PlainRows<T, 8>{px, x_stride, rows, len}, w, m, n, k, out, y_stride, s);
+      else few_rows<T, 1, 2, 1>(PlainRows<T, 8>{px, x_stride, rows, len}, w, m, n, k, out, y_stride, s);
     });
     check(hipGetLastError(), "mx_linear");
     return;
@@ -650,10 +740,90 @@ void launch_mx_linear(int dev, const void* x, const std::string& dtype, int64_t 
   require(aligned(workspace, 16), "mx_linear: workspace aligned to 16 bytes");
   auto codes = static_cast<char*>(workspace);
   auto scales = codes + mx_codes_bytes(m, k);
-  const size_t used = round16(static_cast<size_t>(mx_codes_bytes(m, k) + mx_scales_bytes(m, k)));
   launch_mx_quantize(dev, x, dtype, m, k, x_stride, false, codes, scales, stream);
-  launch_mx_product(dev, codes, scales, w_codes, w_scales, m, n, k, y, dtype, y_stride, codes + used,
-                    workspace_bytes - used, stream);
+  launch_mx_product(dev, codes, scales, w_codes, w_scales, m, n, k, y, dtype, y_stride, codes + mx_bytes(m, k),
+                    workspace_bytes - mx_bytes(m, k), stream);
+}
+
+// ---- training step -------------------------------------------------------------------------------
+// saved: x and w down their columns (rows k, along m and along n). Workspaces: what else is quantised,
+// then the products'.
+size_t mx_linear_train_saved(int64_t m, int64_t n, int64_t k) {
+  check_product(m, n, k, n);
+  return mx_bytes(k, m) + mx_bytes(k, n);
+}
+size_t mx_linear_train_workspace(int64_t m, int64_t n, int64_t k) {
+  return mx_bytes(m, k) + mx_bytes(n, k) + mx_product_workspace(m, n, k);
+}
+
+void launch_mx_linear_train(int dev, const void* x, const std::string& dtype, int64_t x_stride, const void* w,
+                            const std::string& w_dtype, int64_t w_stride, int64_t m, int64_t n, int64_t k, void* y,
+                            int64_t y_stride, void* saved, size_t saved_bytes, void* workspace, size_t workspace_bytes,
+                            void* stream) {
+  const Type t = type_of(dtype, "mx_linear_train: dtype must be bf16|f16|f32");
+  require(m >= 1 && n >= 1, "mx_linear_train: m and n must be >= 1");
+  check_product(m, n, k, y_stride);
+  require(saved && saved_bytes >= mx_linear_train_saved(m, n, k) && aligned(saved, 16) && workspace &&
+              workspace_bytes >= mx_linear_train_workspace(m, n, k) && aligned(workspace, 16),
+          "mx_linear_train: saved and workspace of their sizes, aligned to 16 bytes");
+  auto kept = static_cast<char*>(saved), ws = static_cast<char*>(workspace);
+  const Quantized xq{ws, m, k}, wq{ws + mx_bytes(m, k), n, k}, xt{kept, k, m}, wt{kept + mx_bytes(k, m), k, n};
+  const Source sources[2] = {{x, x_stride, m, k, xq.at, xt.at}, {w, w_stride, n, k, wq.at, wt.at}};
+  const Job j{xq.operand(), wq.operand(), m, n, k, y, y_stride};
+  check_job(j, t);
+  auto s = static_cast<hipStream_t>(stream);
+  const Type tw = type_of(w_dtype, "mx_linear_train: w_dtype must be bf16|f16|f32");
+  check_source(sources[0], t);
+  check_source(sources[1], tw);
+  if (t == tw) {
+    launch_quantize_both(dev, sources, 2, t, s);
+  } else {
+    launch_quantize_both(dev, sources, 1, t, s);
+    launch_quantize_both(dev, sources + 1, 1, tw, s);
+  }
+  const size_t used = static_cast<size_t>(mx_bytes(m, k) + mx_bytes(n, k));
+  launch_products(dev, &j, 1, t, ws + used, workspace_bytes - used, s);
+}
+
+size_t mx_linear_grad_workspace(int64_t m, int64_t n, int64_t k) {
+  check_product(m, n, k, n);
+  const Job jobs[2] = {{{}, {}, m, k, n, nullptr, k}, {{}, {}, n, k, m, nullptr, k}};
+  return mx_bytes(m, n) + mx_bytes(n, m) + products_workspace(jobs, 2);
+}
+
+void launch_mx_linear_grad(int dev, const void* dy, const std::string& dtype, int64_t dy_stride, const void* saved,
+                           int64_t m, int64_t n, int64_t k, void* dx, int64_t dx_stride, void* dw,
+                           const std::string& w_dtype, int64_t dw_stride, void* workspace, size_t workspace_bytes,
+                           void* stream) {
+  const Type t = type_of(dtype, "mx_linear_grad: dtype must be bf16|f16|f32");
+  const Type tw = type_of(w_dtype, "mx_linear_grad: w_dtype must be bf16|f16|f32");
+  require(m >= 1 && n >= 1, "mx_linear_grad: m and n must be >= 1");
+  check_product(m, k, n, dx ? dx_stride : k);
+  check_product(n, k, m, dw ? dw_stride : k);
+  require(saved && aligned(saved, 16) && workspace && workspace_bytes >= mx_linear_grad_workspace(m, n, k) &&
+              aligned(workspace, 16),
+          "mx_linear_grad: saved and workspace of their sizes, aligned to 16 bytes");
+  auto kept = static_cast<char*>(const_cast<void*>(saved)), ws = static_cast<char*>(workspace);
+  const Quantized along{ws, m, n}, down{ws + mx_bytes(m, n), n, m}, xt{kept, k, m}, wt{kept + mx_bytes(k, m), k, n};
+  const Source source{dy, dy_stride, m, n, along.at, down.at};
+  check_source(source, t);
+  const Job jobs[2] = {{along.operand(), wt.operand(), m, k, n, dx, dx_stride}, {down.operand(), xt.operand(), n, k, m, dw, dw_stride}};
+  if (dx) check_job(jobs[0], t);
+  if (dw) check_job(jobs[1], tw);
+  auto s = static_cast<hipStream_t>(stream);
+  const size_t used = static_cast<size_t>(mx_bytes(m, n) + mx_bytes(n, m));
+  auto products = [&](const Job* j, int count, Type type) {
+    launch_products(dev, j, count, type, ws + used, workspace_bytes - used, s);
+  };
+  if (dx && dw) launch_quantize_both(dev, &source, 1, t, s);
+  else if (dx) launch_mx_quantize(dev, dy, dtype, m, n, dy_stride, false, along.at, along.scales(), stream);
+  else if (dw) launch_mx_quantize(dev, dy, dtype, m, n, dy_stride, true, down.at, down.scales(), stream);
+  if (dx && dw && t == tw) {
+    products(jobs, 2, t);
+  } else {
+    if (dx) products(jobs, 1, t);
+    if (dw) products(jobs + 1, 1, tw);
+  }
 }
 
 }  // namespace gpumon_hip

@@ -70,16 +70,33 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const T* __restrict_
 // reading. A workgroup takes 32 rows x 512 columns, whole KiB of a row of a 16-bit type at a time: as they
 // arrive they are quantised along the row, as above, and left in LDS; then each thread takes two columns,
 // neighbours in a 16-bit type (a word of each row), 256 apart in f32.
+// One launch takes up to two matrices.
+struct Both {
+  const void* x;
+  int64_t stride;
+  unsigned rows;
+  int k;
+  Div groups;
+  unsigned blocks;  // workgroups
+  char *row_codes, *row_scales, *col_codes, *col_scales;
+};
+struct TwoBoth {
+  Both of[2];
+};
 template <typename T, bool ROWS>
-__global__ void __launch_bounds__(256) quantize_tile_kernel(const T* __restrict__ x, int64_t stride, unsigned rows,
-                                                            int k, Div groups, char* __restrict__ row_codes,
-                                                            char* __restrict__ row_scales, char* __restrict__ col_codes,
-                                                            char* __restrict__ col_scales) {
+__global__ void __launch_bounds__(256) quantize_tile_kernel(TwoBoth both) {
   constexpr int kWords = 8 / Elem<T>::kPerWord;  // of eight elements
   constexpr int kRow = 64 * kWords;              // words of a row of the tile
   __shared__ __attribute__((aligned(16))) unsigned tile[32 * kRow];
   __shared__ Piece piece[ROWS ? 2 : 1];
-  const unsigned tr = groups.quot(blockIdx.x), g = blockIdx.x - tr * groups.d;
+  const Both& m = both.of[blockIdx.x < both.of[0].blocks ? 0 : 1];
+  const T* x = static_cast<const T*>(m.x);
+  const int64_t stride = m.stride;
+  const unsigned rows = m.rows, bid = blockIdx.x - (blockIdx.x < both.of[0].blocks ? 0 : both.of[0].blocks);
+  const int k = m.k;
+  const Div groups = m.groups;
+  char *row_codes = m.row_codes, *row_scales = m.row_scales, *col_codes = m.col_codes, *col_scales = m.col_scales;
+  const unsigned tr = groups.quot(bid), g = bid - tr * groups.d;
   const unsigned lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   unsigned w[8][kWords];
   with_reach<T>(static_cast<int>(g * 512 + 512), k, [&](auto how) {
@@ -126,10 +143,10 @@ __global__ void __launch_bounds__(256) quantize_tile_kernel(const T* __restrict_
   for (unsigned h = 0; h < 2; ++h) {
     const unsigned col = g * 512 + (Elem<T>::kPerWord == 2 ? threadIdx.x * 2 + h : h * 256 + threadIdx.x);
     const unsigned* e = v + h * (32 / Elem<T>::kPerWord);
-    unsigned m = 0;
+    unsigned top = 0;
 #pragma unroll
-    for (int i = 0; i < 32 / Elem<T>::kPerWord; ++i) m = Elem<T>::amax(m, e[i]);
-    const unsigned byte = scale_byte(Elem<T>::amax_f32(m));
+    for (int i = 0; i < 32 / Elem<T>::kPerWord; ++i) top = Elem<T>::amax(top, e[i]);
+    const unsigned byte = scale_byte(Elem<T>::amax_f32(top));
     const float s = scale_of(byte);
     u32x4 o;
 #pragma unroll
@@ -204,15 +221,36 @@ void check_matrix(const void* data, int64_t rows, int64_t k, int64_t stride, con
 unsigned blocks_for(int64_t n, int64_t per) { return static_cast<unsigned>((n + per - 1) / per); }
 
 template <typename T, bool ROWS>
-void launch_tiles(const T* x, int64_t rows, int64_t k, int64_t stride, char* row_codes, char* row_scales,
-                  char* col_codes, char* col_scales, hipStream_t s) {
-  const unsigned groups = static_cast<unsigned>(mx_groups(k));
-  hipLaunchKernelGGL((quantize_tile_kernel<T, ROWS>), dim3(static_cast<unsigned>(mx_quads(rows) * 4) * groups), dim3(256), 0, s,
-                     x, stride, static_cast<unsigned>(rows), static_cast<int>(k), Div(groups), row_codes, row_scales,
-                     col_codes, col_scales);
+void launch_tiles(const Both* of, int count, hipStream_t s) {
+  TwoBoth both{{of[0], of[count - 1]}};
+  for (Both& m : both.of) m.blocks = static_cast<unsigned>(mx_quads(m.rows) * 4) * m.groups.d;
+  hipLaunchKernelGGL((quantize_tile_kernel<T, ROWS>), dim3(both.of[0].blocks + (count > 1 ? both.of[1].blocks : 0)), dim3(256),
+                     0, s, both);
+}
+Both both_of(const void* x, int64_t rows, int64_t k, int64_t stride, void* rc, void* rs, void* cc, void* cs) {
+  return {x, stride, static_cast<unsigned>(rows), static_cast<int>(k), Div(static_cast<unsigned>(mx_groups(k))), 0,
+          static_cast<char*>(rc), static_cast<char*>(rs), static_cast<char*>(cc), static_cast<char*>(cs)};
 }
 
 }  // namespace
+
+void check_source(const Source& s, Type t) {
+  check_matrix(s.x, s.rows, s.k, s.stride, s.along, s.along, t);
+  require(s.rows >= 1, "mx: rows must be >= 1");
+  check_matrix(s.x, s.k, s.rows, s.rows, s.down, s.down, t);
+}
+void launch_quantize_both(int dev, const Source* sources, int count, Type t, hipStream_t s) {
+  OnDevice on(dev);
+  Both of[2];
+  for (int i = 0; i < count; ++i) {
+    const Source& m = sources[i];
+    const Quantized along{m.along, m.rows, m.k}, down{m.down, m.k, m.rows};
+    of[i] = both_of(m.x, m.rows, m.k, m.stride, along.at, along.scales(), down.at, down.scales());
+  }
+  with_type(t, [&](auto e) { launch_tiles<decltype(e), true>(of, count, s); });
+  check(hipGetLastError(), "mx_quantize_both");
+}
+
 }  // namespace mx
 
 using namespace mx;
@@ -233,7 +271,8 @@ void launch_mx_quantize(int dev, const void* x, const std::string& dtype, int64_
     using T = decltype(e);
     auto px = static_cast<const T*>(x);
     if (by_column) {
-      launch_tiles<T, false>(px, rows, k, stride, nullptr, nullptr, pc, ps, s);
+      const Both of = both_of(x, rows, k, stride, nullptr, nullptr, pc, ps);
+      launch_tiles<T, false>(&of, 1, s);
     } else {
       const unsigned groups = static_cast<unsigned>(mx_groups(k));
       hipLaunchKernelGGL(quantize_rows_kernel<T>, dim3(groups * blocks_for(rows, 16)), dim3(256), 0, s, px, stride,
@@ -251,12 +290,8 @@ void launch_mx_quantize_both(int dev, const void* x, const std::string& dtype, i
   require(rows >= 1, "mx_quantize_both: rows must be >= 1");
   check_matrix(x, k, rows, rows, col_codes, col_scales, t);
   OnDevice on(dev);
-  with_type(t, [&](auto e) {
-    using T = decltype(e);
-    launch_tiles<T, true>(static_cast<const T*>(x), rows, k, stride, static_cast<char*>(row_codes),
-                          static_cast<char*>(row_scales), static_cast<char*>(col_codes), static_cast<char*>(col_scales),
-                          static_cast<hipStream_t>(stream));
-  });
+  const Both of = both_of(x, rows, k, stride, row_codes, row_scales, col_codes, col_scales);
+  with_type(t, [&](auto e) { launch_tiles<decltype(e), true>(&of, 1, static_cast<hipStream_t>(stream)); });
   check(hipGetLastError(), "mx_quantize_both");
 }
 

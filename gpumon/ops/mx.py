@@ -227,7 +227,7 @@ class LinearSaved:
     """What :func:`linear_train` keeps for :func:`linear_grad`: x and w with blocks along the axes that
     the gradients contract over."""
 
-    __slots__ = ("x", "w", "shape", "n", "dtype", "w_dtype", "device")
+    __slots__ = ("buf", "shape", "rows", "n", "k", "dtype", "w_dtype", "device")
 
 
 def linear_train(x, w):
@@ -241,15 +241,25 @@ def linear_train(x, w):
     n, k = w.shape
     if n < 1 or k < 1:
         raise ValueError(f"mx: w is {tuple(w.shape)}: neither size may be 0")
+    dev = x.device
+    x2 = _rows(x if x.dim() == 2 else x.reshape(-1, k))
+    w = _rows(w)
+    m = x2.shape[0]
     saved = LinearSaved()
-    saved.shape, saved.n, saved.dtype, saved.w_dtype, saved.device = tuple(x.shape), n, x.dtype, w.dtype, x.device
-    x2 = x.reshape(-1, k)
-    wq, saved.w = quantize_both(w)
-    if x2.shape[0] == 0:
-        saved.x = None
-        return torch.empty(*x.shape[:-1], n, dtype=x.dtype, device=x.device), saved
-    xq, saved.x = quantize_both(x2)
-    return matmul(xq, wq, x.dtype).view(*x.shape[:-1], n), saved
+    saved.shape, saved.rows, saved.n, saved.k = x.shape, m, n, k
+    saved.dtype, saved.w_dtype, saved.device = x.dtype, w.dtype, dev
+    y = torch.empty(*x.shape[:-1], n, dtype=x.dtype, device=dev)
+    if m == 0:
+        saved.buf = None
+        return y, saved
+    h = hip()
+    size, need = h.mx_linear_train_saved(m, n, k), h.mx_linear_train_workspace(m, n, k)
+    saved.buf = torch.empty(size, dtype=torch.uint8, device=dev)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    h.mx_linear_train(dev.index, x2.data_ptr(), DTYPES[x.dtype], _row_stride(x2), w.data_ptr(), DTYPES[w.dtype],
+                      _row_stride(w), m, n, k, y.data_ptr(), n, saved.buf.data_ptr(), size, ws.data_ptr(), need,
+                      _stream(dev))
+    return y, saved
 
 
 def linear_grad(dy, saved: LinearSaved, need_dx: bool = True, need_dw: bool = True):
@@ -259,25 +269,23 @@ def linear_grad(dy, saved: LinearSaved, need_dx: bool = True, need_dw: bool = Tr
     _check(dy, "dy")
     if not isinstance(saved, LinearSaved):
         raise TypeError(f"mx: saved must come from linear_train, not {type(saved).__name__}")
-    if tuple(dy.shape) != saved.shape[:-1] + (saved.n,):
-        raise ValueError(f"mx: dy is {tuple(dy.shape)}, expected {saved.shape[:-1] + (saved.n,)}")
+    m, n, k, dev = saved.rows, saved.n, saved.k, saved.device
+    if dy.shape[:-1] != saved.shape[:-1] or dy.dim() < 1 or dy.shape[-1] != n:
+        raise ValueError(f"mx: dy is {tuple(dy.shape)}, expected {tuple(saved.shape[:-1]) + (n,)}")
     if dy.dtype != saved.dtype:
         raise TypeError(f"mx: dy is {dy.dtype}, the layer's output {saved.dtype}")
-    if dy.device != saved.device:
-        raise ValueError(f"mx: dy is on {dy.device}, the layer on {saved.device}")
-    k = saved.shape[-1]
-    if saved.x is None:  # no rows
-        return (torch.empty(saved.shape, dtype=saved.dtype, device=saved.device) if need_dx else None,
-                torch.zeros(saved.n, k, dtype=saved.w_dtype, device=saved.device) if need_dw else None)
-    d2 = dy.reshape(-1, saved.n)
-    dx = dw = None
-    if need_dx and need_dw:
-        along, down = quantize_both(d2)
-    else:
-        along = quantize(d2, 1) if need_dx else None
-        down = quantize(d2, 0) if need_dw else None
-    if need_dx:
-        dx = matmul(along, saved.w, saved.dtype).view(saved.shape)
-    if need_dw:
-        dw = matmul(down, saved.x, saved.w_dtype)
+    if dy.device != dev:
+        raise ValueError(f"mx: dy is on {dy.device}, the layer on {dev}")
+    dx = torch.empty(saved.shape, dtype=saved.dtype, device=dev) if need_dx else None
+    if m == 0:
+        return dx, torch.zeros(n, k, dtype=saved.w_dtype, device=dev) if need_dw else None
+    dw = torch.empty(n, k, dtype=saved.w_dtype, device=dev) if need_dw else None
+    if need_dx or need_dw:
+        h = hip()
+        d2 = _rows(dy if dy.dim() == 2 else dy.reshape(-1, n))
+        need = h.mx_linear_grad_workspace(m, n, k)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        h.mx_linear_grad(dev.index, d2.data_ptr(), DTYPES[dy.dtype], _row_stride(d2), saved.buf.data_ptr(), m, n, k,
+                         dx.data_ptr() if need_dx else 0, k, dw.data_ptr() if need_dw else 0, DTYPES[saved.w_dtype], k,
+                         ws.data_ptr(), need, _stream(dev))
     return dx, dw

@@ -295,7 +295,8 @@ def test_linear_with_nan_rows_strides_and_leading_dimensions(mx, m):
 
 
 @pytest.mark.parametrize("dtype,w_dtype", [(BF16, BF16), (F16, F32), (F32, BF16)])
-@pytest.mark.parametrize("m,n,k", [(1, 1, 1), (5, 33, 70), (130, 64, 100), (300, 257, 131)])
+@pytest.mark.parametrize("m,n,k", [(1, 1, 1), (5, 33, 70), (130, 64, 100), (300, 257, 131), (613, 1000, 337), (40, 520, 9000),
+                                   (9000, 70, 80), (1200, 1300, 2100)])
 def test_training_step_against_the_formulas(mx, m, n, k, dtype, w_dtype):
     x, w, dy = values(m, k, dtype, 1), values(n, k, w_dtype, 2), values(m, n, dtype, 3)
     y, saved = mx.linear_train(x, w)

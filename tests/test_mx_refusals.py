@@ -94,3 +94,27 @@ def test_native_linear_refuses_a_small_workspace(H):
     assert need > 0
     with pytest.raises(ValueError, match="workspace"):
         H.mx_linear(0, P, "bf16", 500, P, P, 300, 400, 500, P, 400, P, need - 1)
+
+
+def test_native_training_step_refuses(H):
+    m, n, k = 40, 50, 60
+    saved, ws = H.mx_linear_train_saved(m, n, k), H.mx_linear_train_workspace(m, n, k)
+    ok = dict(dev=0, x=P, dtype="bf16", x_stride=k, w=P, w_dtype="f32", w_stride=k, m=m, n=n, k=k, y=P, y_stride=n, saved=P,
+              saved_bytes=saved, workspace=P, workspace_bytes=ws)
+    for over, match in (({"dtype": "f64"}, "dtype"), ({"w_dtype": "i8"}, "w_dtype"), ({"m": 0}, "m and n"),
+                        ({"n": 0}, "m and n"), ({"k": 0}, "k >= 1"), ({"x_stride": k - 1}, "stride"),
+                        ({"w_stride": k - 1}, "stride"), ({"y_stride": n - 1}, "stride"), ({"x": 0}, "null"),
+                        ({"w": 0}, "null"), ({"y": 0}, "null"), ({"saved": 0}, "sizes"), ({"saved_bytes": saved - 1}, "sizes"),
+                        ({"workspace_bytes": ws - 1}, "sizes"), ({"workspace": P + 8}, "sizes"), ({"w": P + 2}, "aligned"),
+                        ({"x": P + 1}, "aligned"), ({"m": 1 << 28}, "limits")):
+        with pytest.raises(ValueError, match=match):
+            H.mx_linear_train(**{**ok, **over})
+    need = H.mx_linear_grad_workspace(m, n, k)
+    ok = dict(dev=0, dy=P, dtype="bf16", dy_stride=n, saved=P, m=m, n=n, k=k, dx=P, dx_stride=k, dw=P, w_dtype="f32",
+              dw_stride=k, workspace=P, workspace_bytes=need)
+    for over, match in (({"dtype": "f64"}, "dtype"), ({"w_dtype": "i8"}, "w_dtype"), ({"m": 0}, "m and n"),
+                        ({"dy_stride": n - 1}, "stride"), ({"dx_stride": k - 1}, "stride"), ({"dw_stride": k - 1}, "stride"),
+                        ({"dy": 0}, "null"), ({"saved": 0}, "sizes"), ({"saved": P + 4}, "sizes"),
+                        ({"workspace_bytes": need - 1}, "sizes"), ({"dx": P + 1}, "aligned"), ({"dw": P + 2}, "aligned")):
+        with pytest.raises(ValueError, match=match):
+            H.mx_linear_grad(**{**ok, **over})
