@@ -202,7 +202,7 @@ __global__ void __launch_bounds__(64 * WM * WN, RESIDENT * WM * WN / 4) product_
     auto multiply = [&](int from, int to) {
 #pragma unroll
       for (int x = from; x < to; ++x) {
-        const int i = x / FN, j = x % FN;
+        const int i = x / FN, j = i % 2 ? FN - 1 - x % FN : x % FN;  // to and fro: each keeps an operand of the last
         acc[i][j] = mfma16<J>(fb[kNow][j], i < kHead ? fa[i] : ft[kNow][i - kHead], acc[i][j], sb[j], sa[i]);
       }
     };

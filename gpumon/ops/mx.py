@@ -45,14 +45,15 @@ if hasattr(torch._C, "_cuda_getCurrentRawStream"):
 
 
 def _check(t, name: str, ndim=None):
+    if isinstance(t, torch.Tensor) and t.is_cuda and t.dtype in DTYPES and (ndim is None or t.dim() == ndim):
+        return
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"mx: {name} must be a tensor, not {type(t).__name__}")
     if not t.is_cuda:
         raise ValueError(f"mx: {name} must be on a GPU, it is on {t.device}")
     if t.dtype not in DTYPES:
         raise TypeError(f"mx: {name} is {t.dtype}: one of bfloat16, float16, float32")
-    if ndim is not None and t.dim() != ndim:
-        raise ValueError(f"mx: {name} has {t.dim()} dimensions, expected {ndim}")
+    raise ValueError(f"mx: {name} has {t.dim()} dimensions, expected {ndim}")
 
 
 def _check_dtype(dtype):
@@ -61,12 +62,16 @@ def _check_dtype(dtype):
 
 
 def _rows(x):
-    """x (2-D) with its elements next to each other along a row and no overlapping rows (else a copy)."""
-    return x if (x.stride(1) == 1 or x.shape[1] == 1) and x.stride(0) >= x.shape[1] else x.contiguous()
-
-
-def _row_stride(x) -> int:
-    return max(x.stride(0), x.shape[1])
+    """``(x, row stride)`` of a 2-D x with its elements next to each other along a row and no overlapping
+    rows (else of a copy)."""
+    r, c = x.shape
+    s0, s1 = x.stride()
+    if (s1 == 1 or c == 1) and s0 >= c:
+        return x, s0
+    if r == 1 and (s1 == 1 or c == 1):
+        return x, c
+    x = x.contiguous()
+    return x, max(x.stride(0), c)
 
 
 class MxTensor:
@@ -83,10 +88,10 @@ class MxTensor:
         rb = (rows + 15) // 16
         codes = rb * ((k + 127) // 128) * 1024
         self.rows, self.k = rows, k
-        self.buf = torch.empty(codes + rb * ((k + 511) // 512) * 256, dtype=torch.uint8, device=device)
-        self.device = self.buf.device
-        self._codes = self.buf.data_ptr()
-        self._scales = self._codes + codes
+        self.buf = buf = torch.empty(codes + rb * ((k + 511) // 512) * 256, dtype=torch.uint8, device=device)
+        self.device = buf.device
+        self._codes = at = buf.data_ptr()
+        self._scales = at + codes
 
     @property
     def shape(self):
@@ -151,12 +156,12 @@ def quantize(x, axis: int = 1) -> MxTensor:
     down = axis in (0, -2)
     if x.stride(0) == 1 and x.stride(1) >= x.shape[0] > 1:  # a transposed view: the other direction of its base
         x, down = x.t(), not down
-    x = _rows(x)
+    x, stride = _rows(x)
     r, c = x.shape
-    q = MxTensor(c, r, x.device) if down else MxTensor(r, c, x.device)
+    dev = x.device
+    q = MxTensor(c, r, dev) if down else MxTensor(r, c, dev)
     if q.rows:
-        hip().mx_quantize(x.device.index, x.data_ptr(), DTYPES[x.dtype], r, c, _row_stride(x), down, q._codes, q._scales,
-                          _stream(x.device))
+        hip().mx_quantize(dev.index, x.data_ptr(), DTYPES[x.dtype], r, c, stride, down, q._codes, q._scales, _stream(dev))
     return q
 
 
@@ -164,11 +169,12 @@ def quantize_both(x):
     """``(quantize(x, 1), quantize(x, 0))`` from one reading of x."""
     _check(x, "x", 2)
     swap = x.stride(0) == 1 and x.stride(1) >= x.shape[0] > 1
-    x = _rows(x.t() if swap else x)
+    x, stride = _rows(x.t() if swap else x)
     r, c = x.shape
-    along, down = MxTensor(r, c, x.device), MxTensor(c, r, x.device)
-    hip().mx_quantize_both(x.device.index, x.data_ptr(), DTYPES[x.dtype], r, c, _row_stride(x), along._codes,
-                           along._scales, down._codes, down._scales, _stream(x.device))
+    dev = x.device
+    along, down = MxTensor(r, c, dev), MxTensor(c, r, dev)
+    hip().mx_quantize_both(dev.index, x.data_ptr(), DTYPES[x.dtype], r, c, stride, along._codes, along._scales,
+                           down._codes, down._scales, _stream(dev))
     return (down, along) if swap else (along, down)
 
 
@@ -210,16 +216,16 @@ def linear(x, w: MxTensor):
         raise ValueError(f"mx: x is {tuple(x.shape)}, its last size must be the weights' k = {w.k}")
     if x.device != w.device:
         raise ValueError(f"mx: x is on {x.device}, w on {w.device}")
-    x2 = x if x.dim() == 2 else x.reshape(-1, w.k)
-    x2 = _rows(x2)
-    m, n = x2.shape[0], w.rows
-    y = torch.empty(*x.shape[:-1], n, dtype=x.dtype, device=x.device)
-    if y.numel():
-        h, dev = hip(), x.device.index
-        need = h.mx_linear_workspace(m, n, w.k, DTYPES[x.dtype])
-        ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
-        h.mx_linear(dev, x2.data_ptr(), DTYPES[x.dtype], _row_stride(x2), w._codes, w._scales, m, n, w.k, y.data_ptr(),
-                    n, ws.data_ptr() if need else 0, need, _stream(x.device))
+    flat = x.dim() == 2
+    x2, stride = _rows(x if flat else x.reshape(-1, w.k))
+    m, n, dev = x2.shape[0], w.rows, x.device
+    y = torch.empty((m, n) if flat else (*x.shape[:-1], n), dtype=x.dtype, device=dev)
+    if m and n:
+        h, dtype = hip(), DTYPES[x.dtype]
+        need = h.mx_linear_workspace(m, n, w.k, dtype)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        h.mx_linear(dev.index, x2.data_ptr(), dtype, stride, w._codes, w._scales, m, n, w.k, y.data_ptr(), n,
+                    ws.data_ptr() if need else 0, need, _stream(dev))
     return y
 
 
@@ -242,8 +248,8 @@ def linear_train(x, w):
     if n < 1 or k < 1:
         raise ValueError(f"mx: w is {tuple(w.shape)}: neither size may be 0")
     dev = x.device
-    x2 = _rows(x if x.dim() == 2 else x.reshape(-1, k))
-    w = _rows(w)
+    x2, x_stride = _rows(x if x.dim() == 2 else x.reshape(-1, k))
+    w, w_stride = _rows(w)
     m = x2.shape[0]
     saved = LinearSaved()
     saved.shape, saved.rows, saved.n, saved.k = x.shape, m, n, k
@@ -256,9 +262,8 @@ def linear_train(x, w):
     size, need = h.mx_linear_train_saved(m, n, k), h.mx_linear_train_workspace(m, n, k)
     saved.buf = torch.empty(size, dtype=torch.uint8, device=dev)
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    h.mx_linear_train(dev.index, x2.data_ptr(), DTYPES[x.dtype], _row_stride(x2), w.data_ptr(), DTYPES[w.dtype],
-                      _row_stride(w), m, n, k, y.data_ptr(), n, saved.buf.data_ptr(), size, ws.data_ptr(), need,
-                      _stream(dev))
+    h.mx_linear_train(dev.index, x2.data_ptr(), DTYPES[x.dtype], x_stride, w.data_ptr(), DTYPES[w.dtype], w_stride, m,
+                      n, k, y.data_ptr(), n, saved.buf.data_ptr(), size, ws.data_ptr(), need, _stream(dev))
     return y, saved
 
 
@@ -282,10 +287,10 @@ def linear_grad(dy, saved: LinearSaved, need_dx: bool = True, need_dw: bool = Tr
     dw = torch.empty(n, k, dtype=saved.w_dtype, device=dev) if need_dw else None
     if need_dx or need_dw:
         h = hip()
-        d2 = _rows(dy if dy.dim() == 2 else dy.reshape(-1, n))
+        d2, stride = _rows(dy if dy.dim() == 2 else dy.reshape(-1, n))
         need = h.mx_linear_grad_workspace(m, n, k)
         ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        h.mx_linear_grad(dev.index, d2.data_ptr(), DTYPES[dy.dtype], _row_stride(d2), saved.buf.data_ptr(), m, n, k,
+        h.mx_linear_grad(dev.index, d2.data_ptr(), DTYPES[dy.dtype], stride, saved.buf.data_ptr(), m, n, k,
                          dx.data_ptr() if need_dx else 0, k, dw.data_ptr() if need_dw else 0, DTYPES[saved.w_dtype], k,
                          ws.data_ptr(), need, _stream(dev))
     return dx, dw
