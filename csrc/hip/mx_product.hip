@@ -1,6 +1,7 @@
 // MXFP4 product and linear layer (format and layout: mx.h).
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 
 #include "mx_common.h"
 
@@ -518,40 +519,64 @@ int compute_units(int dev) {
 constexpr int64_t kFewRows = 64;
 constexpr int kComputeUnits = 256;  // what the choices between kernels are made for
 
-constexpr int kEnough = kComputeUnits * 4 / 5;  // tiles that fill the chip
-// Which kernel a product takes.
-struct Plan {
-  enum Shape { kFew, k256, k128, k64x128, k64 } shape;
-  unsigned parts, per;  // of k, and groups of quads a part
+// What the tile kernels take, in us, measured on MI355X (products of 2048 and 8192 elements along k, 128 to
+// 2048 tiles): a stage (a quad of k) with at most half, or at most one, tile a compute unit; once some have
+// two; a stage for each tile a compute unit where there are many; and what does not depend on k, alone
+// and for each tile a compute unit.
+struct TileCost {
+  int m, n;
+  bool whole_rounds;  // one tile a compute unit at a time
+  double half, one, two, each, fixed, fixed_each;
 };
-// The largest tiles of which there are enough, over all of a launch's products; false if there are too few
-// of any.
-bool plan_tiles(const Job* jobs, int count, Plan& p) {
-  auto tiles = [&](int64_t tm, int64_t tn) {
-    int64_t t = 0;
-    for (int i = 0; i < count; ++i) t += (jobs[i].m + tm - 1) / tm * ((jobs[i].n + tn - 1) / tn);
-    return t;
-  };
-  bool deep = true, wide = true;
-  for (int i = 0; i < count; ++i) deep &= jobs[i].k > 512, wide &= jobs[i].n > 64;
-  const int64_t big = tiles(256, 256);
-  p.parts = 1;
-  if (deep && big * 5 >= (big + kComputeUnits - 1) / kComputeUnits * kComputeUnits * 4) p.shape = Plan::k256;
-  else if (tiles(128, 128) >= kEnough) p.shape = Plan::k128;
-  else if (wide && tiles(64, 128) >= kEnough) p.shape = Plan::k64x128;
-  else return p.shape = Plan::k64, false;
-  return true;
+constexpr TileCost kTiles[] = {
+    {256, 256, true, 0.62, 0.81, 0, 0.82, 6, 5},   {256, 128, true, 0.35, 0.43, 0, 0.46, 8, 1.5},
+    {128, 128, false, 0.22, 0.24, 0.37, 0.24, 6, 1}, {64, 128, false, 0.16, 0.19, 0.28, 0.15, 5.3, 0.5},
+    {64, 64, false, 0.13, 0.13, 0.195, 0.098, 4.8, 0.5},
+};
+struct Plan {
+  enum Shape { k256, k256x128, k128, k64x128, k64, kFew } shape;  // as in kTiles
+  unsigned parts, per;  // of k, and groups of quads a part
+  double us;
+};
+Plan plan_tiles(const Job* jobs, int count) {
+  Plan best{Plan::k64, 1, 0, 1e30};
+  const int64_t groups = count == 1 ? mx_groups(jobs[0].k) : 0;
+  for (int shape = 0; shape < 5; ++shape) {
+    const TileCost& c = kTiles[shape];
+    int64_t total = 0;
+    double stages = 0, longest = 0;
+    for (int i = 0; i < count; ++i) {
+      const int64_t t = (jobs[i].m + c.m - 1) / c.m * ((jobs[i].n + c.n - 1) / c.n);
+      const double q = static_cast<double>(mx_groups(jobs[i].k)) * 4;
+      total += t;
+      stages += q * static_cast<double>(t);
+      longest = std::max(longest, q);
+    }
+    stages /= static_cast<double>(total);
+    auto us = [&](int64_t tiles, double len) {
+      const double x = static_cast<double>(tiles) / kComputeUnits, rounds = std::ceil(x);
+      const double stage = x <= 0.5 ? c.half : x <= 1 ? c.one : c.whole_rounds ? c.each * rounds : std::max(c.two, c.each * x);
+      return c.fixed + c.fixed_each * (c.whole_rounds ? rounds : x) + len * stage;
+    };
+    const double one = us(total, total <= kComputeUnits ? longest : stages);
+    if (one < best.us) best = {static_cast<Plan::Shape>(shape), 1, static_cast<unsigned>(groups), one};
+    if (shape != Plan::k64 || count > 1 || total >= kComputeUnits) continue;
+    // k in parts: their sums, written and read, and a launch more
+    for (int64_t parts = 2; parts <= 8 && parts * 2 <= groups; ++parts) {
+      const int64_t per = (groups + parts - 1) / parts, some = (groups + per - 1) / per;
+      const double t = us(total * some, static_cast<double>(per) * 4) + 3 + static_cast<double>(some * jobs[0].m * jobs[0].n) * 8 / 4e6;
+      if (t < best.us) best = {Plan::k64, static_cast<unsigned>(some), static_cast<unsigned>(per), t};
+    }
+  }
+  return best;
 }
 Plan plan(const Job& j) {
-  const int64_t groups = mx_groups(j.k), small = (j.m + 63) / 64 * ((j.n + 63) / 64);
-  Plan p{Plan::kFew, 1, static_cast<unsigned>(groups)};
-  if (j.m <= 32 || (j.m <= kFewRows && small < 192)) return p;
-  if (!plan_tiles(&j, 1, p) && small * 2 <= kComputeUnits && groups >= 16) {
-    const int64_t parts = std::min<int64_t>(kComputeUnits / small, groups / 4), per = (groups + parts - 1) / parts;
-    p.parts = static_cast<unsigned>((groups + per - 1) / per);
-    p.per = static_cast<unsigned>(per);
-  }
-  return p;
+  const int64_t small = (j.m + 63) / 64 * ((j.n + 63) / 64);
+  // few rows: the weights stream by (from the same measurements, 3.5 us and 5 TB/s, less with more rows)
+  if (j.m <= 32 || (j.m <= kFewRows && small < 192))
+    return {Plan::kFew, 1, static_cast<unsigned>(mx_groups(j.k)),
+            3.5 + static_cast<double>(j.n) * static_cast<double>(mx_quads(j.k)) * 68 * (1 + static_cast<double>(j.m) / 64) / 5e6};
+  return plan_tiles(&j, 1);
 }
 
 void check_product(int64_t m, int64_t n, int64_t k, int64_t stride) {
@@ -630,6 +655,7 @@ void run_jobs(int dev, Job* jobs, int count, const Plan& p, Type t, void* worksp
         break;
       }
       case Plan::k256: run_tiles<T, 8, 4, 2, 4, 1>(dev, jobs, count, p, s); break;
+      case Plan::k256x128: run_tiles<T, 4, 4, 4, 2, 1>(dev, jobs, count, p, s); break;
       case Plan::k128: run_tiles<T, 4, 4, 2, 2, 2>(dev, jobs, count, p, s); break;
       case Plan::k64x128: run_tiles<T, 2, 4, 2, 2, 2>(dev, jobs, count, p, s); break;
       case Plan::k64:
@@ -652,8 +678,8 @@ void run_jobs(int dev, Job* jobs, int count, const Plan& p, Type t, void* worksp
 
 }  // namespace
 
-// Up to two products of one result type; together where each would take whole tiles by itself, so that
-// the chip is filled once, else one after the other with the workspace in common.
+// Up to two products of one result type, together or one after the other (the workspace in common),
+// whichever should take less.
 size_t products_workspace(const Job* jobs, int count) {
   size_t need = 0;
   for (int i = 0; i < count; ++i) need = std::max(need, job_workspace(jobs[i]));
@@ -673,9 +699,9 @@ void launch_products(int dev, const Job* jobs, int count, Type t, void* workspac
   OnDevice on(dev);
   Plan p = plan(todo[0]);
   if (n == 2) {
-    const Plan q = plan(todo[1]);
-    if (p.shape != Plan::kFew && q.shape != Plan::kFew && p.parts == 1 && q.parts == 1) {
-      plan_tiles(todo, 2, p);
+    const Plan q = plan(todo[1]), both = plan_tiles(todo, 2);
+    if (both.us <= p.us + q.us) {
+      p = both;
     } else {
       run_jobs(dev, todo, 1, p, t, workspace, s);
       todo[0] = todo[1];

@@ -193,7 +193,7 @@ PRODUCTS = [(1, 1, 1), (1, 16, 32), (1, 1000, 4096), (2, 33, 64), (7, 130, 129),
             (17, 48, 640), (31, 1411, 256), (33, 65, 300), (64, 64, 128), (65, 257, 1025), (100, 100, 100),
             (128, 128, 256), (129, 300, 384), (200, 1000, 2500), (256, 256, 256), (257, 511, 768), (300, 260, 130),
             (512, 512, 1152), (513, 1030, 2048), (777, 1411, 2999), (1024, 2048, 640), (2100, 1100, 300), (1, 70000, 96),
-            (5000, 3, 200), (3, 5, 100000), (40, 40, 20000), (70, 66, 9000), (130, 200, 8192), (500, 300, 33000), (300, 20, 12345)]
+            (5000, 3, 200), (3, 5, 100000), (40, 40, 20000), (70, 66, 9000), (130, 200, 8192), (500, 300, 33000), (300, 20, 12345), (2000, 2100, 300), (3600, 1029, 1300)]
 
 
 @pytest.mark.parametrize("m,n,k", PRODUCTS)
