@@ -29,9 +29,9 @@ struct Piece {
     codes[at(quad, block, row, lane & 3)] = byte == 255 ? 0u : codes8<T>(w, scale_of(byte));
     if ((lane & 3) == 0) scales[(block * 16 + row) * 4 + quad] = static_cast<unsigned char>(byte);
   }
-  // By 256 threads, to row block rb and group g.
+  // By four waves, to row block rb and group g.
   __device__ __forceinline__ void store(char* out, char* out_scales, unsigned rb, unsigned g, unsigned quads, unsigned groups) const {
-    const unsigned lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const unsigned lane = threadIdx.x & 63, wave = threadIdx.x >> 6 & 3;
     if (g * 4 + wave < quads)
       *reinterpret_cast<u32x4*>(out + (static_cast<size_t>(rb) * quads + g * 4 + wave) * 1024 + lane * 16) =
           *reinterpret_cast<const u32x4*>(&codes[at(wave, lane >> 4, lane & 15, 0)]);
@@ -68,8 +68,7 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const T* __restrict_
 
 // Blocks down a column (the result's rows are x's columns), and with ROWS along the rows too, from one
 // reading. A workgroup takes 32 rows x 512 columns, whole KiB of a row of a 16-bit type at a time: as they
-// arrive they are quantised along the row, as above, and left in LDS; then each thread takes two columns,
-// neighbours in a 16-bit type (a word of each row), 256 apart in f32.
+// arrive they are quantised along the row, as above, and left in LDS; then each thread takes a column.
 // One launch takes up to two matrices.
 struct Both {
   const void* x;
@@ -84,7 +83,7 @@ struct TwoBoth {
   Both of[2];
 };
 template <typename T, bool ROWS>
-__global__ void __launch_bounds__(256) quantize_tile_kernel(TwoBoth both) {
+__global__ void __launch_bounds__(512) quantize_tile_kernel(TwoBoth both) {
   constexpr int kWords = 8 / Elem<T>::kPerWord;  // of eight elements
   constexpr int kRow = 64 * kWords;              // words of a row of the tile
   __shared__ __attribute__((aligned(16))) unsigned tile[32 * kRow];
@@ -98,16 +97,16 @@ __global__ void __launch_bounds__(256) quantize_tile_kernel(TwoBoth both) {
   char *row_codes = m.row_codes, *row_scales = m.row_scales, *col_codes = m.col_codes, *col_scales = m.col_scales;
   const unsigned tr = groups.quot(bid), g = bid - tr * groups.d;
   const unsigned lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  unsigned w[8][kWords];
+  unsigned w[4][kWords];
   with_reach<T>(static_cast<int>(g * 512 + 512), k, [&](auto how) {
 #pragma unroll
-    for (unsigned i = 0; i < 8; ++i)
-      load8<decltype(how)::value>(x + static_cast<int64_t>(min(tr * 32 + wave * 8 + i, rows - 1)) * stride,
+    for (unsigned i = 0; i < 4; ++i)
+      load8<decltype(how)::value>(x + static_cast<int64_t>(min(tr * 32 + wave * 4 + i, rows - 1)) * stride,
                                   static_cast<int>(g * 512 + lane * 8), k, w[i]);
   });
 #pragma unroll
-  for (unsigned i = 0; i < 8; ++i) {
-    const unsigned r = wave * 8 + i;
+  for (unsigned i = 0; i < 4; ++i) {
+    const unsigned r = wave * 4 + i;
     if (tr * 32 + r >= rows)
       for (unsigned& v : w[i]) v = 0;
 #pragma unroll
@@ -117,47 +116,42 @@ __global__ void __launch_bounds__(256) quantize_tile_kernel(TwoBoth both) {
   }
   __syncthreads();
   if constexpr (ROWS) {
-    const unsigned quads = (static_cast<unsigned>(k) + 127) / 128;
-#pragma unroll
-    for (unsigned h = 0; h < 2; ++h)
-      if (tr * 2 + h < (rows + 15) / 16) piece[h].store(row_codes, row_scales, tr * 2 + h, g, quads, groups.d);
+    const unsigned h = wave >> 2;
+    if (tr * 2 + h < (rows + 15) / 16)
+      piece[h].store(row_codes, row_scales, tr * 2 + h, g, (static_cast<unsigned>(k) + 127) / 128, groups.d);
   }
-  unsigned v[64 / Elem<T>::kPerWord];  // 32 elements of one column after 32 of the other
+  // a column a thread; of a 16-bit type its half of the words that hold two, even columns first
+  constexpr int kColWords = 32 / Elem<T>::kPerWord;
+  unsigned v[kColWords];
+  unsigned c = threadIdx.x;
+  if constexpr (Elem<T>::kPerWord == 2) {
+    const unsigned pair = threadIdx.x & 255, odd = threadIdx.x >> 8;
+    c = pair * 2 + odd;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    if constexpr (Elem<T>::kPerWord == 2) {
-      const unsigned a = tile[2 * i * kRow + threadIdx.x], b = tile[(2 * i + 1) * kRow + threadIdx.x];
-      v[i] = (a & 0xffffu) | (b << 16);
-      v[16 + i] = (a >> 16) | (b & 0xffff0000u);
-    } else {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        v[2 * i + h] = tile[(2 * i + h) * kRow + threadIdx.x];
-        v[32 + 2 * i + h] = tile[(2 * i + h) * kRow + 256 + threadIdx.x];
-      }
+    for (int i = 0; i < 16; ++i) {
+      const unsigned a = tile[2 * i * kRow + pair], b = tile[(2 * i + 1) * kRow + pair];
+      v[i] = __builtin_amdgcn_perm(b, a, odd ? 0x07060302u : 0x05040100u);
     }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = tile[i * kRow + threadIdx.x];
   }
+  unsigned top = 0;
+#pragma unroll
+  for (unsigned e : v) top = Elem<T>::amax(top, e);
+  const unsigned byte = scale_byte(Elem<T>::amax_f32(top));
+  const float s = scale_of(byte);
+  u32x4 o;
+#pragma unroll
+  for (int p = 0; p < 4; ++p) o[p] = byte == 255 ? 0u : codes8<T>(v + p * kWords, s);
   // row tr of tiles is block tr % 4 of quad tr / 4 down the columns
-  const unsigned quads = (rows + 127) / 128, q = tr >> 2, b = tr & 3, col_groups = (quads + 3) / 4;
-#pragma unroll
-  for (unsigned h = 0; h < 2; ++h) {
-    const unsigned col = g * 512 + (Elem<T>::kPerWord == 2 ? threadIdx.x * 2 + h : h * 256 + threadIdx.x);
-    const unsigned* e = v + h * (32 / Elem<T>::kPerWord);
-    unsigned top = 0;
-#pragma unroll
-    for (int i = 0; i < 32 / Elem<T>::kPerWord; ++i) top = Elem<T>::amax(top, e[i]);
-    const unsigned byte = scale_byte(Elem<T>::amax_f32(top));
-    const float s = scale_of(byte);
-    u32x4 o;
-#pragma unroll
-    for (int p = 0; p < 4; ++p) o[p] = byte == 255 ? 0u : codes8<T>(e + p * kWords, s);
-    if (col < (static_cast<unsigned>(k) + 15) / 16 * 16) {
-      *reinterpret_cast<u32x4*>(col_codes + (static_cast<size_t>(col >> 4) * quads + q) * 1024 + b * 256 + (col & 15) * 16) = o;
-      char* sp = col_scales + (static_cast<size_t>(col >> 4) * col_groups + (q >> 2)) * 256 + b * 64 + (col & 15) * 4;
-      sp[q & 3] = static_cast<char>(byte);
-      if (q + 1 == quads)
-        for (unsigned j = (q & 3) + 1; j < 4; ++j) sp[j] = 0;
-    }
+  const unsigned quads = (rows + 127) / 128, q = tr >> 2, b = tr & 3, col_groups = (quads + 3) / 4, col = g * 512 + c;
+  if (col < (static_cast<unsigned>(k) + 15) / 16 * 16) {
+    *reinterpret_cast<u32x4*>(col_codes + (static_cast<size_t>(col >> 4) * quads + q) * 1024 + b * 256 + (col & 15) * 16) = o;
+    char* sp = col_scales + (static_cast<size_t>(col >> 4) * col_groups + (q >> 2)) * 256 + b * 64 + (col & 15) * 4;
+    sp[q & 3] = static_cast<char>(byte);
+    if (q + 1 == quads)
+      for (unsigned j = (q & 3) + 1; j < 4; ++j) sp[j] = 0;
   }
 }
 
@@ -224,7 +218,7 @@ template <typename T, bool ROWS>
 void launch_tiles(const Both* of, int count, hipStream_t s) {
   TwoBoth both{{of[0], of[count - 1]}};
   for (Both& m : both.of) m.blocks = static_cast<unsigned>(mx_quads(m.rows) * 4) * m.groups.d;
-  hipLaunchKernelGGL((quantize_tile_kernel<T, ROWS>), dim3(both.of[0].blocks + (count > 1 ? both.of[1].blocks : 0)), dim3(256),
+  hipLaunchKernelGGL((quantize_tile_kernel<T, ROWS>), dim3(both.of[0].blocks + (count > 1 ? both.of[1].blocks : 0)), dim3(512),
                      0, s, both);
 }
 Both both_of(const void* x, int64_t rows, int64_t k, int64_t stride, void* rc, void* rs, void* cc, void* cs) {
