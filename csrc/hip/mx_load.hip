@@ -41,6 +41,8 @@ MxLoad::~MxLoad() { stop(); }
 
 void MxLoad::start() {
   if (running_) return;
+  stop();  // a thread that ended by an error is still to be joined
+  failed_ = false;
   check(hipSetDevice(dev_), "hipSetDevice");
   try {
     hipStream_t s;

@@ -33,6 +33,14 @@ __device__ __forceinline__ void load_lds(Buffer b, unsigned offset, unsigned uni
   __builtin_amdgcn_raw_ptr_buffer_load_lds(b, (LdsVoid*)lds, 16, static_cast<int>(offset), static_cast<int>(uniform), 0, 0);
 }
 
+// All waves of the workgroup meet, after waits of their own: a barrier that no access to memory crosses,
+// but that, unlike __syncthreads, waits for no loads still on their way to LDS.
+__device__ __forceinline__ void meet() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
 template <int S>
 using Int = std::integral_constant<int, S>;
 
@@ -180,7 +188,7 @@ __global__ void __launch_bounds__(64 * WM * WN, RESIDENT * WM * WN / 4) product_
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) load_chunk(i, t * 1024, t);
   __builtin_amdgcn_s_waitcnt(wait_imm(3 * kLoads, false));
-  __builtin_amdgcn_s_barrier();
+  meet();
   read_scales(0);
 #pragma unroll
   for (int x = 0; x < kHead; ++x) fa[x] = read_a(x, 0);
@@ -195,7 +203,7 @@ __global__ void __launch_bounds__(64 * WM * WN, RESIDENT * WM * WN / 4) product_
     // stage g * 4 + J + 1 is here, for every wave, and every wave has read the one before it
     constexpr int kAfter = 2 * kLoads + (J == 1 || J == 2 ? kScaleLoads : 0);
     __builtin_amdgcn_s_waitcnt(wait_imm(kAfter, true));
-    __builtin_amdgcn_s_barrier();
+    meet();
     __builtin_amdgcn_sched_barrier(0);
     constexpr int kNow = J & 1, kNext = kNow ^ 1, kSlot = (J + 1) & 3;
     const bool last = g + 1 == groups;  // then the next tile's loads

@@ -64,6 +64,8 @@ def _check_dtype(dtype):
 def _rows(x):
     """``(x, row stride)`` of a 2-D x with its elements next to each other along a row and no overlapping
     rows (else of a copy)."""
+    if x.is_neg():  # a lazily negated view: its memory holds other values
+        x = x.resolve_neg()
     r, c = x.shape
     s0, s1 = x.stride()
     if (s1 == 1 or c == 1) and s0 >= c:
@@ -137,6 +139,10 @@ class MxTensor:
         codes = self.codes.permute(0, 3, 1, 2, 4).reshape(r16, -1)[:self.rows, :blocks * 16]
         scales = self.scales.permute(0, 3, 1, 4, 2).reshape(r16, -1)[:self.rows, :blocks]
         return codes.contiguous(), scales.contiguous()
+
+    def record_stream(self, stream) -> None:
+        """As ``torch.Tensor.record_stream``: before it is dropped while work on another stream uses it."""
+        self.buf.record_stream(stream)
 
     def __repr__(self):
         return f"MxTensor({self.rows} x {self.k}, {self.device})"
@@ -234,6 +240,11 @@ class LinearSaved:
     the gradients contract over."""
 
     __slots__ = ("buf", "shape", "rows", "n", "k", "dtype", "w_dtype", "device")
+
+    def record_stream(self, stream) -> None:
+        """As ``torch.Tensor.record_stream``."""
+        if self.buf is not None:
+            self.buf.record_stream(stream)
 
 
 def linear_train(x, w):
