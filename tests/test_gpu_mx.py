@@ -447,3 +447,174 @@ def test_offsets_past_32_bits(mx):
     y = mx.matmul(mx.quantize(x[-40:, :200]), mx.quantize(x[:, :200].contiguous()), BF16)
     assert_product(y[:, -40:], ref_round(x[-40:, :200]), ref_round(x[-40:, :200]))
     assert not y[:, :-40].any()
+
+
+def test_first_calls_of_a_process_inside_a_capture(mx):
+    """Kernels are loaded and the device asked for its size by the first call, which may be a captured one."""
+    import subprocess
+    import sys
+
+    code = """
+import torch
+from gpumon.ops import mx
+g0 = torch.Generator().manual_seed(1)
+x = torch.randn(300, 260, generator=g0).to(torch.bfloat16).cuda()
+w = torch.randn(400, 260, generator=g0).to(torch.bfloat16).cuda()
+dy = torch.randn(300, 400, generator=g0).to(torch.bfloat16).cuda()
+torch.cuda.synchronize()
+def step():
+    y, saved = mx.linear_train(x, w)
+    dx, dw = mx.linear_grad(dy, saved)
+    q = mx.quantize(w)
+    return [y, dx, dw, mx.linear(x[:1], q), mx.linear(x[:20], q), mx.dequantize(q), mx.matmul(q, q)]
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    out = step()
+want = step()
+for _ in range(3):
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(out, want))
+print("ok")
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=100)
+    assert r.returncode == 0 and r.stdout.strip() == "ok", r.stderr[-2000:]
+
+
+def test_two_threads_at_once(mx):
+    import threading
+
+    xs = [values(200 + 30 * i, 700, BF16, i) for i in range(2)]
+    w = mx.quantize(values(300, 700, BF16, 9))
+    want = [mx.linear(x, w) for x in xs]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(50):
+                y = mx.linear(xs[i], w)
+                torch.cuda.current_stream().synchronize()
+                if not torch.equal(y, want[i]):
+                    bad.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+
+
+def test_one_tensor_in_both_places(mx):
+    x = values(90, 200, BF16, 1)
+    v = ref_round(x)
+    q = mx.quantize(x)
+    assert_product(mx.matmul(q, q, F32), v, v)
+    y, saved = mx.linear_train(x, x)
+    dx, dw = mx.linear_grad(y, saved)
+    assert_product(y, v, v)
+    assert_product(dx, ref_round(y), ref_round(x.t()))
+    assert_product(dw, ref_round(y.t()), ref_round(x.t()))
+
+
+def test_training_step_with_nan_and_infinities(mx):
+    x, w, dy = values(70, 130, BF16, 1, True), values(50, 130, F32, 2, True), values(70, 50, BF16, 3, True)
+    y, saved = mx.linear_train(x, w)
+    dx, dw = mx.linear_grad(dy, saved)
+    assert_product(y, ref_round(x), ref_round(w))
+    assert_product(dx, ref_round(dy), ref_round(w.t()))
+    assert_product(dw, ref_round(dy.t()), ref_round(x.t()))
+
+
+def test_views_that_share_or_negate_their_elements(mx):
+    base = values(1, 700, BF16, 2)
+    w = values(60, 200, BF16, 3)
+    wq, wv = mx.quantize(w), ref_round(w)
+    for x in (base[:, :200].expand(40, 200), base.as_strided((40, 200), (3, 1)), base.as_strided((40, 200), (1, 3)),
+              base.as_strided((40, 200), (0, 0)), torch._neg_view(values(40, 200, BF16, 4))):
+        assert_quantized(mx.quantize(x), x)
+        assert_quantized(mx.quantize(x, 0), x.t())
+        assert_product(mx.linear(x, wq), ref_round(x), wv)
+        y, saved = mx.linear_train(x, w)
+        assert_product(y, ref_round(x), wv)
+        dy = x[:, :60]
+        dx, dw = mx.linear_grad(dy, saved)
+        assert_product(dx, ref_round(dy), ref_round(w.t()))
+        assert_product(dw, ref_round(dy.t()), ref_round(x.t()))
+
+
+def test_nothing_to_do(mx):
+    q0, q = mx.quantize(torch.empty(0, 70, device="cuda")), mx.quantize(values(5, 70, F32, 1))
+    assert mx.dequantize(q0).shape == (0, 70)
+    assert mx.matmul(q0, q).shape == (0, 5) and mx.matmul(q, q0).shape == (5, 0)
+    assert mx.linear(values(3, 70, BF16, 1), q0).shape == (3, 0)
+    assert mx.linear(torch.empty(2, 0, 70, device="cuda"), q).shape == (2, 0, 5)
+    for bad in (lambda: mx.quantize(torch.empty(4, 0, device="cuda")), lambda: mx.quantize(torch.empty(0, 4, device="cuda"), 0),
+                lambda: mx.quantize_both(torch.empty(0, 4, device="cuda")),
+                lambda: mx.linear_train(values(3, 4, BF16), torch.empty(0, 4, dtype=BF16, device="cuda"))):
+        with pytest.raises(ValueError):
+            bad()
+
+
+def test_refusals_on_the_gpu(mx):
+    x, w = values(3, 70, BF16, 1), values(5, 70, BF16, 2)
+    q = mx.quantize(w)
+    for bad in (lambda: mx.quantize(x[0]), lambda: mx.quantize(x, 2), lambda: mx.linear(x[:, :69], q),
+                lambda: mx.linear(values(1, 1, BF16)[0, 0], q), lambda: mx.matmul(q, mx.quantize(x[:, :69])),
+                lambda: mx.linear_train(x, w[:, :69]), lambda: mx.linear_grad(x, mx.linear_train(x, w)[1])):
+        with pytest.raises(ValueError):
+            bad()
+    for bad in (lambda: mx.quantize(x.double()), lambda: mx.linear(x.int(), q), lambda: mx.linear(x, w),
+                lambda: mx.linear_grad(values(3, 5, F16), mx.linear_train(x, w)[1])):
+        with pytest.raises(TypeError):
+            bad()
+
+
+def test_weights_dropped_while_another_stream_uses_them(mx):
+    """record_stream: memory of a quantised matrix is not given out again before the other stream is done."""
+    x = values(64, 4096, BF16, 1)
+    w = values(4096, 4096, BF16, 2)
+    want = mx.linear(x, mx.quantize(w))
+    s = torch.cuda.Stream()
+    for _ in range(5):
+        q = mx.quantize(w)
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            for _ in range(10):
+                y = mx.linear(x, q)
+        q.record_stream(s)
+        del q
+        torch.empty(9 << 20, dtype=torch.uint8, device="cuda").fill_(255)
+        torch.cuda.synchronize()
+        assert torch.equal(y, want)
+
+
+def test_products_past_32_bits(mx):
+    """Operands and results of more than 2^32 bytes, with whole numbers so that every sum is exact."""
+    g = torch.Generator(device="cuda").manual_seed(7)
+
+    def whole(rows, k):
+        v = torch.randint(-3, 4, (rows, k), generator=g, device="cuda").to(BF16)
+        v[:, ::32] = 6  # one scale everywhere
+        return v
+
+    n, k = 66000, 135000  # 4.5e9 bytes of codes
+    w = torch.zeros(n, k, dtype=BF16, device="cuda")
+    w[:64], w[-64:] = whole(64, k), whole(64, k)
+    q = mx.quantize(w)
+    ends = torch.cat([w[:64], w[-64:]]).float()
+    del w
+    for m in (1, 5, 40, 200):
+        x = whole(m, k)
+        y = mx.matmul(mx.quantize(x), q, F32)
+        assert torch.equal(torch.cat([y[:, :64], y[:, -64:]], 1), x.float() @ ends.t()), m
+        assert not y[:, 64:-64].any()
+        if m in (1, 40):
+            assert torch.equal(mx.linear(x.float(), q)[:, -64:], y[:, -64:])
+    del q, y
+    m, n, k = 70000, 33000, 64  # 4.6e9 bytes of results
+    a, b = whole(m, k), whole(n, k)
+    y = mx.matmul(mx.quantize(a), mx.quantize(b), F32)
+    for rows in (slice(0, 300), slice(35000, 35200), slice(m - 300, m)):
+        assert torch.equal(y[rows], a[rows].float() @ b.float().t())
