@@ -151,7 +151,8 @@ __device__ __forceinline__ void with_reach(int end, int k, F f) {
   else f(std::integral_constant<Reach, Reach::tiny>{});
 }
 
-// 16 bytes written once, past the caches (6.3 TB/s where plain stores came to 3.5), aligned or not.
+// 16 bytes written once, past the caches, aligned or not (8192 x 8192 dequantised to bf16: 6.2 TB/s, plain
+// stores 4.8; a product of 8192 x 8000 x 512 35.5 us, plain stores 37.2 to 38.1).
 template <typename T>
 __device__ __forceinline__ void store16(T* to, const T* v) {
   struct __attribute__((packed, aligned(sizeof(T)))) Out {

@@ -81,11 +81,21 @@ __device__ __forceinline__ void hold() {
   }
 }
 
-// WM x WN waves, FM x FN chunks of 16 x 16 results each. The stages (a quad of every chunk of the tile)
-// go through LDS in four slots, loaded three stages ahead, without a break from one tile to the next;
-// a stage's operands are read into registers while the one before multiplies, so that the matrix
-// instructions wait for nothing but the barrier (Order). b's rows take the instruction's A side: a lane's four
-// sums are neighbours in a row of c.
+// WM x WN waves, FM x FN chunks of 16 x 16 results each: sums of 128 elements a matrix instruction in f32,
+// scales applied by it, rounded once at the end. The stages (a quad of every chunk of the tile) go
+// through LDS in four slots, loaded three stages ahead, without a break from one tile to the next; a
+// stage's operands are read into registers while the one before multiplies, so that the matrix
+// instructions wait for nothing but the barrier (Order). b's rows take the instruction's A side: a lane's
+// four sums are neighbours in a row of c.
+//
+// The larger the tile the less each element is read: 256 x 256 results need 32 KiB a stage for 64 matrix
+// instructions a SIMD. Eight waves of 128 x 64, since four of 128 x 128, which read a third less from LDS,
+// were no faster (8192^3 236 to 254 us, these 240 to 261). What bounds large products is most likely the
+// power their operands' bits take: the same launch takes 212 to 261 us on random ones (5.2 to 4.2 PFLOP/s)
+// and 157 to 167 on zeros; matrix instructions alone, on random registers, come to 7.25 PFLOP/s. About 10
+// us of a launch are its first loads and last stores (one tile a compute unit, fitted over k). Smaller
+// tiles are for fewer results, so that every compute unit has one (kTiles has what each takes).
+//
 // One launch takes up to two products, the second's tiles after the first's.
 // SPLIT: the tiles' columns are taken `parts` times, each time with `per` of k's groups of quads, and each
 // part's sums go to a matrix of its own.
@@ -311,7 +321,8 @@ __global__ void __launch_bounds__(64 * WM * WN, RESIDENT * WM * WN / 4) product_
   __builtin_amdgcn_s_waitcnt(wait_imm(0, true));  // no load may arrive after the workgroup's memory is given back
 }
 
-// c = the parts' sums, added up in their order; four columns a thread.
+// c = the parts' sums, added up in their order (no atomics: the same result every time); four columns a
+// thread. 206 x 491 results of 4 parts: 5.0 us, next to 6.4 for the parts.
 template <typename T>
 __global__ void __launch_bounds__(256) product_sum_kernel(const float* __restrict__ sums, unsigned parts, unsigned m,
                                                           unsigned n, T* __restrict__ c, int64_t stride, Div quarters) {
@@ -340,7 +351,9 @@ __global__ void __launch_bounds__(256) product_sum_kernel(const float* __restric
 }
 
 // ---- few rows ----------------------------------------------------------------------------------
-// x has at most 16 FM rows: the weights' bytes are the work. A workgroup takes R row blocks of b (16 R
+// x has at most 16 FM rows: the weights' bytes are the work (8192 x 8192 weights, 36 MB: a row 7.2 us,
+// 5.0 TB/s, 64 rows, whose codes each workgroup reads too, 11.8; a row on 28672 x 8192 5.7 TB/s). A workgroup
+// takes R row blocks of b (16 R
 // results a row of x), its waves whole groups of quads in turn, straight from memory to registers,
 // U groups a wave in flight; the waves' sums meet in LDS in a fixed order. Sources of x: rows
 // quantised before, or plain rows that each wave quantises for its own groups.

@@ -41,7 +41,10 @@ struct Piece {
   }
 };
 
-// Blocks along a row. A wave takes 512 elements of four rows, their loads in flight together.
+// Blocks along a row: amax, the scale's exponent and the codes as in mx.h. A wave takes 512 elements of four
+// rows, their loads in flight together; a workgroup ends up with whole chunks and scale words and writes
+// them 16 bytes a lane. Bound by memory: 8192 x 8192 bf16 (134 MB read, 36 written) 28.7 us, 5.9 TB/s,
+// where a plain copy of 1 GiB reaches 6.55; one token of 8192 2.8 us, a launch's least.
 template <typename T>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const T* __restrict__ x, int64_t stride, unsigned rows,
                                                             int k, Div groups, unsigned quads, char* __restrict__ codes,
@@ -69,6 +72,10 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const T* __restrict_
 // Blocks down a column (the result's rows are x's columns), and with ROWS along the rows too, from one
 // reading. A workgroup takes 32 rows x 512 columns, whole KiB of a row of a 16-bit type at a time: as they
 // arrive they are quantised along the row, as above, and left in LDS; then each thread takes a column.
+// Both directions of 8192 x 8192 bf16: 40 us, 5.1 TB/s (57 with a wave's loads one after the other, where
+// 128 x 128 elements a workgroup took 53). A scale word's four bytes come from four workgroups, each
+// storing its own. Bound by memory, and by the chain of its steps where there are few workgroups: both
+// directions of two matrices of 4096 x 8192 in one launch 35 us, 5.9 TB/s; of 613 x 1000 f16 4.7 us.
 // One launch takes up to two matrices.
 struct Both {
   const void* x;
@@ -155,6 +162,10 @@ __global__ void __launch_bounds__(512) quantize_tile_kernel(TwoBoth both) {
   }
 }
 
+// Codes times scale, rounded to T (exact in bf16 and f32). The same pieces the other way round; stores past
+// the caches: 8192 x 8192 to bf16 25.4 us, 6.7 TB/s (in a graph of several 27.3, and 35.3 with plain
+// stores). Rows that do not start on a cache line leave parts of lines at each piece's ends: 4099 x 2053 to
+// f32 9.9 us, 3.9 TB/s.
 template <typename T>
 __global__ void __launch_bounds__(256) dequantize_kernel(const char* __restrict__ codes, const char* __restrict__ scales,
                                                          unsigned rows, int k, Div groups, unsigned quads,
