@@ -303,9 +303,12 @@ __global__ void __launch_bounds__(64 * WM * WN, RESIDENT * WM * WN / 4) product_
           __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         }
     };
+    // A store instruction leaves up to four pieces of a row; past the caches where they are whole lines
+    // (8192 x 8064 x 512 to bf16 35 us, through them 38 to 39; 8192 x 8016 71 and 49; 8192 x 8001 102 and 55).
+    const bool past = __builtin_amdgcn_readfirstlane(whole_lines(out, stride));
     if (__builtin_amdgcn_readfirstlane(row0 + FM * 16 <= m && col0 + FN * 16 <= n)) {
       leave([&](unsigned row, unsigned col, const T* v) {
-        store16(out + static_cast<int64_t>(row) * stride + col, v);
+        store16(out + static_cast<int64_t>(row) * stride + col, v, past);
       });
     } else {
       leave([&](unsigned row, unsigned col, const T* v) {
