@@ -13,8 +13,8 @@
 // A lane's operand of v_mfma_scale_f32_16x16x128_f8f6f4 is one block of one row (lane l: row l & 15,
 // block l >> 4), so a wave's operand is one "chunk" of 1 KiB in lane order, and the scale words of
 // four such steps are 256 bytes in lane order, the instruction picking the step's byte. Memory, LDS
-// and registers hold the same order: every transfer is contiguous, with no bank conflicts and no
-// shuffles.
+// and registers hold the same order: every transfer is contiguous, without shuffles and with few
+// bank conflicts (3 % of the LDS cycles of an 8192^3 product).
 #pragma once
 
 #include <cstddef>
