@@ -89,11 +89,15 @@ class MxTensor:
             raise ValueError(f"mx: a quantised matrix needs rows >= 0 and k >= 1, not {rows} x {k}")
         rb = (rows + 15) // 16
         codes = rb * ((k + 127) // 128) * 1024
-        self.rows, self.k = rows, k
-        self.buf = buf = torch.empty(codes + rb * ((k + 511) // 512) * 256, dtype=torch.uint8, device=device)
-        self.device = buf.device
+        self._hold(torch.empty(codes + rb * ((k + 511) // 512) * 256, dtype=torch.uint8, device=device), rows, k, codes)
+
+    def _hold(self, buf, rows: int, k: int, codes: int):
+        self.rows, self.k, self.buf, self.device = rows, k, buf, buf.device
         self._codes = at = buf.data_ptr()
         self._scales = at + codes
+
+    def __reduce__(self):  # a copied or loaded matrix has its addresses from its own buffer
+        return _remake, (self.buf, self.rows, self.k)
 
     @property
     def shape(self):
@@ -148,9 +152,24 @@ class MxTensor:
         return f"MxTensor({self.rows} x {self.k}, {self.device})"
 
 
+def _remake(buf, rows: int, k: int) -> MxTensor:
+    rb = (rows + 15) // 16
+    codes, scales = rb * ((k + 127) // 128) * 1024, rb * ((k + 511) // 512) * 256
+    if buf.dtype != torch.uint8 or buf.shape != (codes + scales,) or not buf.is_contiguous():
+        raise ValueError(f"mx: a {rows} x {k} matrix needs a buffer of {codes + scales} uint8, not {tuple(buf.shape)} {buf.dtype}")
+    q = MxTensor.__new__(MxTensor)
+    q._hold(buf, rows, k, codes)
+    return q
+
+
 def _check_mx(q, name: str):
     if not isinstance(q, MxTensor):
         raise TypeError(f"mx: {name} must be an MxTensor, not {type(q).__name__}")
+
+
+def _check_gpu(q, name: str):
+    if not q.buf.is_cuda:
+        raise ValueError(f"mx: {name} must be on a GPU, it is on {q.device}")
 
 
 def quantize(x, axis: int = 1) -> MxTensor:
@@ -188,6 +207,7 @@ def dequantize(q: MxTensor, dtype=torch.float32):
     """What q stands for, [rows, k]; exact in bf16 and f32, rounded in f16."""
     _check_mx(q, "q")
     _check_dtype(dtype)
+    _check_gpu(q, "q")
     out = torch.empty(q.rows, q.k, dtype=dtype, device=q.device)
     if q.rows:
         hip().mx_dequantize(q.device.index, q._codes, q._scales, q.rows, q.k, out.data_ptr(), DTYPES[dtype], q.k,
@@ -204,6 +224,7 @@ def matmul(a: MxTensor, b: MxTensor, dtype=torch.bfloat16):
         raise ValueError(f"mx: a is {a.rows} x {a.k} and b {b.rows} x {b.k}: the second sizes differ")
     if a.device != b.device:
         raise ValueError(f"mx: a is on {a.device}, b on {b.device}")
+    _check_gpu(a, "a")
     c = torch.empty(a.rows, b.rows, dtype=dtype, device=a.device)
     if c.numel():
         h, dev = hip(), a.device.index
@@ -292,6 +313,8 @@ def linear_grad(dy, saved: LinearSaved, need_dx: bool = True, need_dw: bool = Tr
         raise TypeError(f"mx: dy is {dy.dtype}, the layer's output {saved.dtype}")
     if dy.device != dev:
         raise ValueError(f"mx: dy is on {dy.device}, the layer on {dev}")
+    if m and saved.buf.device != dev:  # loaded from a file to somewhere else
+        raise ValueError(f"mx: saved is on {saved.buf.device}, the layer on {dev}")
     dx = torch.empty(saved.shape, dtype=saved.dtype, device=dev) if need_dx else None
     if m == 0:
         return dx, torch.zeros(n, k, dtype=saved.w_dtype, device=dev) if need_dw else None

@@ -618,3 +618,29 @@ def test_products_past_32_bits(mx):
     y = mx.matmul(mx.quantize(a), mx.quantize(b), F32)
     for rows in (slice(0, 300), slice(35000, 35200), slice(m - 300, m)):
         assert torch.equal(y[rows], a[rows].float() @ b.float().t())
+
+
+def test_copied_and_loaded_matrices_and_saved_layers(mx):
+    """Copies that outlive what they were made from, whose memory holds something else by then."""
+    import copy
+    import io
+
+    x, w = torch.randn(5, 300, device="cuda").bfloat16(), torch.randn(70, 300, device="cuda").bfloat16()
+    dy = torch.randn(5, 70, device="cuda").bfloat16()
+    q = mx.quantize(w)
+    y, (want, saved) = mx.linear(x, q), mx.linear_train(x, w)
+    grads = mx.linear_grad(dy, saved)
+    file = io.BytesIO()
+    torch.save((q, saved), file)
+    file.seek(0)
+    copies = [copy.deepcopy((q, saved)), torch.load(file, weights_only=False)]
+    q.buf.fill_(255)
+    saved.buf.fill_(255)
+    del q
+    for cq, cs in copies:
+        assert torch.equal(mx.linear(x, cq), y)
+        for a, b in zip(mx.linear_grad(dy, cs), grads):
+            assert torch.equal(a, b)
+    cs.buf = cs.buf.cpu()
+    with pytest.raises(ValueError, match="saved is on cpu"):
+        mx.linear_grad(dy, cs)

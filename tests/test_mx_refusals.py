@@ -50,6 +50,41 @@ def test_products_of_other_sizes_are_refused(mx):
         mx.dequantize(a, torch.int32)
 
 
+def _copies(q):
+    import copy
+    import io
+    import pickle
+
+    file = io.BytesIO()
+    torch.save(q, file)
+    file.seek(0)
+    return copy.deepcopy(q), copy.copy(q), pickle.loads(pickle.dumps(q)), torch.load(file, weights_only=False)
+
+
+@pytest.mark.parametrize("rows,k", [(1, 1), (3, 64), (17, 1337)])
+def test_a_copied_matrix_uses_its_own_memory(mx, rows, k):
+    q = mx.MxTensor(rows, k, "cpu")
+    q.buf.copy_(torch.arange(q.buf.numel()).to(torch.uint8))
+    for c in _copies(q):
+        assert c.shape == q.shape and c.device == q.device
+        assert c._codes == c.buf.data_ptr() and c._scales - c._codes == q._scales - q._codes
+        assert torch.equal(c.codes, q.codes) and torch.equal(c.scales, q.scales)
+
+
+def test_a_matrix_is_not_rebuilt_from_another_buffer(mx):
+    q = mx.MxTensor(17, 1337, "cpu")
+    remake, (buf, rows, k) = q.__reduce__()
+    for bad in (buf[:-1], buf.view(torch.int8), torch.cat((buf, buf))[::2]):
+        with pytest.raises(ValueError, match="buffer"):
+            remake(bad, rows, k)
+
+
+def test_matrices_off_the_gpu_are_refused(mx):
+    a, b = mx.MxTensor(3, 64, "cpu"), mx.MxTensor(5, 64, "cpu")
+    for f in (lambda: mx.matmul(a, b), lambda: mx.dequantize(a)):
+        with pytest.raises(ValueError, match="on a GPU"):
+            f()
+
 P = 1 << 20  # an aligned address that nothing here reaches
 
 
