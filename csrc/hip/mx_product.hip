@@ -622,9 +622,11 @@ void check_product(int64_t m, int64_t n, int64_t k, int64_t stride) {
 }
 
 // Whether a linear layer's rows are quantised by the workgroups that multiply them, each for itself, or
-// once by a launch before. The launch costs 2.5 us; on the way, each workgroup reads and quantises all of
-// x: 400 KB of it a compute unit, over its workgroups one after the other, take about as long (bf16, 8
-// rows: 8192 x 8192 weights 10.4 us on the way, 12.6 with the launch; 4096 x 28672 19.6 and 18.5).
+// once by a launch before. The launch costs 2 to 3 us; on the way, each workgroup reads and quantises all of
+// x: 400 KB of it a compute unit, over its workgroups one after the other, take about as long. In us, on the
+// way and with the launch: bf16, 8 rows, 8192 x 8192 weights 9.5 and 11.5, 4096 x 28672 16.5 and 16.8, 28672 x
+// 8192 25.0 and 25.6; f32, 4096 x 28672, 2 rows 14.7 and 16.9, 5 rows 20.2 and 16.9. Where it is wrong by most:
+// two f32 rows on 28672 x 8192, which it takes on the way, 28.9 and 25.2.
 bool quantise_on_the_way(int64_t m, int64_t n, int64_t k, int size) {
   const int64_t blocks = (n + 15) / 16;
   // row blocks in hand at once: two workgroups a compute unit for up to four rows, else one of one or two
