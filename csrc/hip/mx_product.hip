@@ -23,14 +23,15 @@ __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c, unsigned sa, 
 // s_waitcnt with a vmcnt and, if lgkm0, lgkmcnt(0).
 constexpr int wait_imm(int vm, bool lgkm0) { return (vm & 15) | ((vm >> 4) << 14) | (7 << 4) | ((lgkm0 ? 0 : 15) << 8); }
 
-// Buffers: a uniform base, offsets of 32 bits of which one is uniform; past `size` reads give zeros.
+// Buffers: a uniform base, an offset of 32 bits a lane; past `size` reads give zeros. The whole offset is the
+// lane's: an instruction's uniform offset is not counted in its check against `size`.
 typedef __amdgpu_buffer_rsrc_t Buffer;
 __device__ __forceinline__ Buffer buffer(const char* base, unsigned size) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base), 0, static_cast<int>(size), 0x00020000);
 }
 // 16 bytes a lane to LDS, lane after lane.
-__device__ __forceinline__ void load_lds(Buffer b, unsigned offset, unsigned uniform, char* lds) {
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(b, (LdsVoid*)lds, 16, static_cast<int>(offset), static_cast<int>(uniform), 0, 0);
+__device__ __forceinline__ void load_lds(Buffer b, unsigned offset, char* lds) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(b, (LdsVoid*)lds, 16, static_cast<int>(offset), 0, 0, 0);
 }
 
 // All waves of the workgroup meet, after waits of their own: a barrier that no access to memory crosses,
@@ -126,7 +127,7 @@ __global__ void __launch_bounds__(64 * WM * WN, RESIDENT * WM * WN / 4) product_
   unsigned soff[kScaleLoads];  // four chunks' scales a load, 16 lanes each; TM is a multiple of 4
   // Where the loads come from: chunk x of a tile, a's TM first. Row blocks past the end read the last one
   // instead, and what comes of them is not stored. Past the last tile, and past the last quad, zeros come
-  // without a read: four steps at a time are taken, and scales there are zeros too.
+  // without a read (load_lds): four steps at a time are taken, and scales there are zeros too.
   auto aim = [&](bool any, const Product& p, unsigned tm, unsigned tn) {
     const unsigned rbm = (p.m + 15) / 16, rbn = (p.n + 15) / 16, quads = p.quads, all_groups = (quads + 3) / 4;
     unsigned g0 = 0;
@@ -153,12 +154,12 @@ __global__ void __launch_bounds__(64 * WM * WN, RESIDENT * WM * WN / 4) product_
     }
   };
   auto load_chunk = [&](int i, unsigned at, int slot) {
-    load_lds(src[i], lane * 16, at, lds + slot * kStage + (wave * kLoads + i) * 1024);
+    load_lds(src[i], lane * 16 + at, lds + slot * kStage + (wave * kLoads + i) * 1024);
   };
   auto load_scales = [&](unsigned g, unsigned half) {
 #pragma unroll
     for (int i = 0; i < kScaleLoads; ++i)
-      load_lds(ssrc[i], soff[i], g * 256, lds + 4 * kStage + half * kScales + (wave * kScaleLoads + i) * 1024 % kScales);
+      load_lds(ssrc[i], soff[i] + g * 256, lds + 4 * kStage + half * kScales + (wave * kScaleLoads + i) * 1024 % kScales);
   };
 
   constexpr Order<FM, FN, kLoads> order;
