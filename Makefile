@@ -55,12 +55,9 @@ $(BIN): $(CORE_OBJ) build/obj/exporter_main.o
 	$(CXX) -o $@ $^ $(LIBS)
 
 # HIP kernels + their pybind11 wrapper in one hipcc-built extension (gfx950 only).
-# Packed f32 arithmetic is off: some of its forms have given wrong results now and then. Except in the
-# 16x16x32 burn, whose waves' residency changes with the code that adds up its sums after the loop: without
-# packed adds 54 % of the wave slots are held on MI355X instead of 94 %, and the K1 probe no longer queues
-# behind it.
-HIPFLAGS16 := --offload-arch=$(GPUMON_ARCH) -O3 -std=c++17 -fPIC -fvisibility=hidden -Icsrc
-HIPFLAGS  := $(HIPFLAGS16) -Xclang -target-feature -Xclang -packed-fp32-ops
+# Packed f32 arithmetic is off: some of its forms have given wrong results now and then.
+NO_PACKED := -Xclang -target-feature -Xclang -packed-fp32-ops
+HIPFLAGS  := --offload-arch=$(GPUMON_ARCH) -O3 -std=c++17 -fPIC -fvisibility=hidden -Icsrc $(NO_PACKED)
 build/obj/hip/kernels.o: csrc/hip/kernels.hip $(HIP_HDR)
 	@mkdir -p $(dir $@)
 	$(HIPCC) $(HIPFLAGS) -c $< -o $@
@@ -71,7 +68,7 @@ build/obj/hip/kernels.o: csrc/hip/kernels.hip $(HIP_HDR)
 BURN16_FLAGS := -mllvm -amdgpu-mfma-vgpr-form
 build/obj/hip/burn16.o: csrc/hip/burn16.hip $(HIP_HDR)
 	@mkdir -p $(dir $@)
-	$(HIPCC) $(HIPFLAGS16) $(BURN16_FLAGS) -c $< -o $@
+	$(HIPCC) $(HIPFLAGS) $(BURN16_FLAGS) -c $< -o $@
 
 build/obj/bindings/hip_module.o: csrc/bindings/hip_module.cpp $(HIP_HDR)
 	@mkdir -p $(dir $@)
@@ -129,7 +126,7 @@ bin/hsa_stages: tools/hsa_stages.cpp
 	$(CXX) -O2 -std=c++17 -Wall -I$(ROCM)/include $< -L$(ROCM)/lib -lhsa-runtime64 -Wl,-rpath,$(ROCM)/lib -o $@
 bin/perf_snapshot_probe: tools/perf_snapshot_probe.hip
 	@mkdir -p bin
-	$(HIPCC) --offload-arch=$(GPUMON_ARCH) -O2 $< -o $@
+	$(HIPCC) --offload-arch=$(GPUMON_ARCH) -O2 $(NO_PACKED) $< -o $@
 
 clean:
 	rm -rf build bin lib gpumon/_core*.so gpumon/_hip*.so gpumon/_pmc*.so
@@ -155,7 +152,7 @@ build/obj/plugins/probe_plugin.o: csrc/plugins/probe_plugin.cpp csrc/plugins/ond
 PROBECO := build/obj/hip/probe_$(GPUMON_ARCH).hsaco
 $(PROBECO): csrc/hip/probe_co.hip $(HIP_HDR)
 	@mkdir -p $(dir $@)
-	$(HIPCC) --offload-arch=$(GPUMON_ARCH) --offload-device-only --no-gpu-bundle-output -O3 -std=c++17 -Icsrc $< -o $@
+	$(HIPCC) --offload-arch=$(GPUMON_ARCH) --offload-device-only --no-gpu-bundle-output -O3 -std=c++17 -Icsrc $(NO_PACKED) $< -o $@
 build/obj/plugins/probe_hsa.o: csrc/plugins/probe_hsa.cpp csrc/plugins/probe_hsa.h $(HIP_HDR) $(PROBECO)
 	@mkdir -p $(dir $@)
 	$(CXX) -O2 -std=c++17 -fPIC -fvisibility=hidden -Wall -Wextra -I$(ROCM)/include \

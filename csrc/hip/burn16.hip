@@ -4,6 +4,7 @@
 // burn in kernels.hip keeps its AGPR form (the VGPR form cost it 94 -> 82 % MFMA busy, measured).
 #include <hip/hip_runtime.h>
 
+#include "burn_common.h"
 #include "hip_api.h"
 
 namespace gpumon_hip {
@@ -36,16 +37,18 @@ __global__ void __launch_bounds__(256) mfma_burn16_kernel(const __bf16* __restri
   // named accumulators (an array of vectors made the compiler rotate AGPRs inside the loop)
   f32x4 c0 = {0.f, 0.f, 0.f, 0.f}, c1 = {1.f, 0.f, 0.f, 0.f}, c2 = {2.f, 0.f, 0.f, 0.f}, c3 = {3.f, 0.f, 0.f, 0.f};
   f32x4 c4 = {4.f, 0.f, 0.f, 0.f}, c5 = {5.f, 0.f, 0.f, 0.f}, c6 = {6.f, 0.f, 0.f, 0.f}, c7 = {7.f, 0.f, 0.f, 0.f};
-  for (int i = 0; i < iters; ++i) {
-    c0 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, bv, c0, 0, 0, 0);
-    c1 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, bv, c1, 0, 0, 0);
-    c2 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, bv, c2, 0, 0, 0);
-    c3 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, bv, c3, 0, 0, 0);
-    c4 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, bv, c4, 0, 0, 0);
-    c5 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, bv, c5, 0, 0, 0);
-    c6 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, bv, c6, 0, 0, 0);
-    c7 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, bv, c7, 0, 0, 0);
-  }
+  hold_slots(iters, [&](int count) {
+    for (int i = 0; i < count; ++i) {
+      c0 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, bv, c0, 0, 0, 0);
+      c1 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, bv, c1, 0, 0, 0);
+      c2 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, bv, c2, 0, 0, 0);
+      c3 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, bv, c3, 0, 0, 0);
+      c4 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, bv, c4, 0, 0, 0);
+      c5 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, bv, c5, 0, 0, 0);
+      c6 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, bv, c6, 0, 0, 0);
+      c7 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(av, bv, c7, 0, 0, 0);
+    }
+  });
   const f32x4 t = c0 + c1 + c2 + c3 + c4 + c5 + c6 + c7;
   const float s = t[0] + t[1] + t[2] + t[3];
   if (lane == 0) out[blockIdx.x * 4 + (threadIdx.x >> 6)] = s;

@@ -8,6 +8,7 @@
 #include <stdexcept>
 #include <string>
 
+#include "burn_common.h"
 #include "hip_api.h"
 
 namespace gpumon_hip {
@@ -104,16 +105,18 @@ __global__ void __launch_bounds__(256) burn_kernel(float* __restrict__ out, int 
   using Acc = typename Op<K>::Acc;
   const int lane = threadIdx.x & 63;
   Acc c0 = {}, c1 = {}, c2 = {}, c3 = {}, c4 = {}, c5 = {}, c6 = {}, c7 = {};
-  for (int i = 0; i < iters; ++i) {
-    c0 = Op<K>::run(c0, lane);
-    c1 = Op<K>::run(c1, lane);
-    c2 = Op<K>::run(c2, lane);
-    c3 = Op<K>::run(c3, lane);
-    c4 = Op<K>::run(c4, lane);
-    c5 = Op<K>::run(c5, lane);
-    c6 = Op<K>::run(c6, lane);
-    c7 = Op<K>::run(c7, lane);
-  }
+  hold_slots(iters, [&](int count) {
+    for (int i = 0; i < count; ++i) {
+      c0 = Op<K>::run(c0, lane);
+      c1 = Op<K>::run(c1, lane);
+      c2 = Op<K>::run(c2, lane);
+      c3 = Op<K>::run(c3, lane);
+      c4 = Op<K>::run(c4, lane);
+      c5 = Op<K>::run(c5, lane);
+      c6 = Op<K>::run(c6, lane);
+      c7 = Op<K>::run(c7, lane);
+    }
+  });
   const Acc t = c0 + c1 + c2 + c3 + c4 + c5 + c6 + c7;
   if (lane == 0) out[blockIdx.x * 4 + (threadIdx.x >> 6)] = static_cast<float>(t[0] + t[1] + t[2] + t[3]);
 }
