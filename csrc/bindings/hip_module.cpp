@@ -80,6 +80,7 @@ PYBIND11_MODULE(_hip, m) {
   }, py::arg("dev"), py::arg("codes"), py::arg("scales"), py::arg("rows"), py::arg("k"), py::arg("out"),
      py::arg("dtype"), py::arg("stride"), py::arg("stream") = 0);
   m.def("mx_product_workspace", &mx_product_workspace, py::arg("m"), py::arg("n"), py::arg("k"));
+  m.def("mx_product_kernel", &mx_product_kernel, py::arg("m"), py::arg("n"), py::arg("k"));
   m.def("mx_product", [](int dev, uintptr_t a_codes, uintptr_t a_scales, uintptr_t b_codes, uintptr_t b_scales,
                          int64_t m, int64_t n, int64_t k, uintptr_t c, const std::string& dtype, int64_t stride,
                          uintptr_t workspace, size_t workspace_bytes, uintptr_t stream) {
@@ -89,6 +90,7 @@ PYBIND11_MODULE(_hip, m) {
      py::arg("n"), py::arg("k"), py::arg("c"), py::arg("dtype"), py::arg("stride"), py::arg("workspace") = 0,
      py::arg("workspace_bytes") = 0, py::arg("stream") = 0);
   m.def("mx_linear_workspace", &mx_linear_workspace, py::arg("m"), py::arg("n"), py::arg("k"), py::arg("dtype"));
+  m.def("mx_linear_kernel", &mx_linear_kernel, py::arg("m"), py::arg("n"), py::arg("k"), py::arg("dtype"));
   m.def("mx_linear", [](int dev, uintptr_t x, const std::string& dtype, int64_t x_stride, uintptr_t w_codes,
                         uintptr_t w_scales, int64_t m, int64_t n, int64_t k, uintptr_t y, int64_t y_stride,
                         uintptr_t workspace, size_t workspace_bytes, uintptr_t stream) {

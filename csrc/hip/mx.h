@@ -52,11 +52,16 @@ void launch_mx_dequantize(int dev, const void* codes, const void* scales, int64_
                           const std::string& dtype, int64_t stride, void* stream);
 // c [m, n] = a [m, k] b [n, k]^T, sums in 32 bits, rounded once. workspace: mx_product_workspace bytes.
 size_t mx_product_workspace(int64_t m, int64_t n, int64_t k);
+// The kernel that these sizes take: a tile's "256x256" to "64x64", "64x64/3" with k in three parts, or "few16" to
+// "few64x2" for few rows.
+std::string mx_product_kernel(int64_t m, int64_t n, int64_t k);
 void launch_mx_product(int dev, const void* a_codes, const void* a_scales, const void* b_codes, const void* b_scales,
                        int64_t m, int64_t n, int64_t k, void* c, const std::string& dtype, int64_t stride,
                        void* workspace, size_t workspace_bytes, void* stream);
 // y [m, n] = Q(x) w^T: x [m, k] in `dtype`, quantised here; y has the same type.
 size_t mx_linear_workspace(int64_t m, int64_t n, int64_t k, const std::string& dtype);
+// The product's kernel as above, or "way1" to "way8x2" where it quantises x on the way.
+std::string mx_linear_kernel(int64_t m, int64_t n, int64_t k, const std::string& dtype);
 void launch_mx_linear(int dev, const void* x, const std::string& dtype, int64_t x_stride, const void* w_codes,
                       const void* w_scales, int64_t m, int64_t n, int64_t k, void* y, int64_t y_stride,
                       void* workspace, size_t workspace_bytes, void* stream);

@@ -570,7 +570,8 @@ constexpr TileCost kTiles[] = {
     {64, 64, false, 0.13, 0.13, 0.195, 0.098, 4.8, 0.5},
 };
 struct Plan {
-  enum Shape { k256, k256x128, k128, k64x128, k64, kFew } shape;  // as in kTiles
+  // tiles as in kTiles, then the most rows of the few-rows kernel, x2 with two row blocks of b a workgroup
+  enum Shape { k256, k256x128, k128, k64x128, k64, kFew16, kFew32, kFew32x2, kFew64, kFew64x2 } shape;
   unsigned parts, per;  // of k, and groups of quads a part
   double us;
 };
@@ -609,10 +610,19 @@ Plan plan_tiles(const Job* jobs, int count) {
 Plan plan(const Job& j) {
   const int64_t small = (j.m + 63) / 64 * ((j.n + 63) / 64);
   // few rows: the weights stream by (from the same measurements, 3.5 us and 5 TB/s, less with more rows)
+  const bool narrow = j.n <= 16 * kComputeUnits;  // a row block a workgroup fills the chip better than two
   if (j.m <= 32 || (j.m <= kFewRows && small < 192))
-    return {Plan::kFew, 1, static_cast<unsigned>(mx_groups(j.k)),
+    return {j.m <= 16   ? Plan::kFew16
+            : j.m <= 32 ? narrow ? Plan::kFew32 : Plan::kFew32x2
+            : narrow    ? Plan::kFew64
+                        : Plan::kFew64x2, 1, static_cast<unsigned>(mx_groups(j.k)),
             3.5 + static_cast<double>(j.n) * static_cast<double>(mx_quads(j.k)) * 68 * (1 + static_cast<double>(j.m) / 64) / 5e6};
   return plan_tiles(&j, 1);
+}
+
+std::string name_of(const Plan& p) {
+  const char* names[] = {"256x256", "256x128", "128x128", "64x128", "64x64", "few16", "few32", "few32x2", "few64", "few64x2"};
+  return p.parts > 1 ? "64x64/" + std::to_string(p.parts) : names[p.shape];
 }
 
 void check_product(int64_t m, int64_t n, int64_t k, int64_t stride) {
@@ -628,11 +638,13 @@ void check_product(int64_t m, int64_t n, int64_t k, int64_t stride) {
 // way and with the launch: bf16, 8 rows, 8192 x 8192 weights 9.5 and 11.5, 4096 x 28672 16.5 and 16.8, 28672 x
 // 8192 25.0 and 25.6; f32, 4096 x 28672, 2 rows 14.7 and 16.9, 5 rows 20.2 and 16.9. Where it is wrong by most:
 // two f32 rows on 28672 x 8192, which it takes on the way, 28.9 and 25.2.
-bool quantise_on_the_way(int64_t m, int64_t n, int64_t k, int size) {
+enum class Way { launch, one, four, eight, eight_x2 };  // the launch before, or the most rows on the way
+Way way_of(int64_t m, int64_t n, int64_t k, int size) {
   const int64_t blocks = (n + 15) / 16;
   // row blocks in hand at once: two workgroups a compute unit for up to four rows, else one of one or two
   const int64_t at_once = m > 4 && blocks <= kComputeUnits ? kComputeUnits : 2 * kComputeUnits;
-  return m <= 8 && m * k * size * ((blocks + at_once - 1) / at_once) <= 400000;
+  if (m > 8 || m * k * size * ((blocks + at_once - 1) / at_once) > 400000) return Way::launch;
+  return m == 1 ? Way::one : m <= 4 ? Way::four : n <= 16 * kComputeUnits ? Way::eight : Way::eight_x2;
 }
 
 }  // namespace
@@ -679,19 +691,16 @@ void run_jobs(int dev, Job* jobs, int count, const Plan& p, Type t, void* worksp
   with_type(t, [&](auto e) {
     using T = decltype(e);
     Job& j = jobs[0];
+    auto rows = [&] {
+      return QuantizedRows{j.a.codes, j.a.scales, static_cast<unsigned>(mx_quads(j.k)),
+                           static_cast<unsigned>(mx_groups(j.k)), static_cast<unsigned>(mx_row_blocks(j.m))};
+    };
     switch (p.shape) {
-      case Plan::kFew: {
-        const QuantizedRows x{j.a.codes, j.a.scales, static_cast<unsigned>(mx_quads(j.k)),
-                              static_cast<unsigned>(mx_groups(j.k)), static_cast<unsigned>(mx_row_blocks(j.m))};
-        auto out = static_cast<T*>(j.c);
-        const bool narrow = j.n <= 16 * kComputeUnits;  // a row block a workgroup fills the chip better than two
-        if (j.m <= 16) few_rows<T, 1, 1, 2>(x, j.b, j.m, j.n, j.k, out, j.stride, s);
-        else if (j.m <= 32 && narrow) few_rows<T, 2, 1, 2>(x, j.b, j.m, j.n, j.k, out, j.stride, s);
-        else if (j.m <= 32) few_rows<T, 2, 2, 2>(x, j.b, j.m, j.n, j.k, out, j.stride, s);
-        else if (narrow) few_rows<T, 4, 1, 1>(x, j.b, j.m, j.n, j.k, out, j.stride, s);
-        else few_rows<T, 4, 2, 2>(x, j.b, j.m, j.n, j.k, out, j.stride, s);
-        break;
-      }
+      case Plan::kFew16: few_rows<T, 1, 1, 2>(rows(), j.b, j.m, j.n, j.k, static_cast<T*>(j.c), j.stride, s); break;
+      case Plan::kFew32: few_rows<T, 2, 1, 2>(rows(), j.b, j.m, j.n, j.k, static_cast<T*>(j.c), j.stride, s); break;
+      case Plan::kFew32x2: few_rows<T, 2, 2, 2>(rows(), j.b, j.m, j.n, j.k, static_cast<T*>(j.c), j.stride, s); break;
+      case Plan::kFew64: few_rows<T, 4, 1, 1>(rows(), j.b, j.m, j.n, j.k, static_cast<T*>(j.c), j.stride, s); break;
+      case Plan::kFew64x2: few_rows<T, 4, 2, 2>(rows(), j.b, j.m, j.n, j.k, static_cast<T*>(j.c), j.stride, s); break;
       case Plan::k256: run_tiles<T, 8, 4, 2, 4, 1>(dev, jobs, count, p, s); break;
       case Plan::k256x128: run_tiles<T, 4, 4, 4, 2, 1>(dev, jobs, count, p, s); break;
       case Plan::k128: run_tiles<T, 4, 4, 2, 2, 2>(dev, jobs, count, p, s); break;
@@ -758,6 +767,11 @@ size_t mx_product_workspace(int64_t m, int64_t n, int64_t k) {
   return job_workspace(Job{{}, {}, m, n, k, nullptr, n});
 }
 
+std::string mx_product_kernel(int64_t m, int64_t n, int64_t k) {
+  check_product(m, n, k, n);
+  return name_of(plan(Job{{}, {}, m, n, k, nullptr, n}));
+}
+
 void launch_mx_product(int dev, const void* a_codes, const void* a_scales, const void* b_codes, const void* b_scales,
                        int64_t m, int64_t n, int64_t k, void* c, const std::string& dtype, int64_t stride,
                        void* workspace, size_t workspace_bytes, void* stream) {
@@ -768,8 +782,15 @@ void launch_mx_product(int dev, const void* a_codes, const void* a_scales, const
 
 size_t mx_linear_workspace(int64_t m, int64_t n, int64_t k, const std::string& dtype) {
   check_product(m, n, k, n);
-  if (quantise_on_the_way(m, n, k, size_of(type_of(dtype, "mx_linear: dtype must be bf16|f16|f32")))) return 0;
+  if (way_of(m, n, k, size_of(type_of(dtype, "mx_linear: dtype must be bf16|f16|f32"))) != Way::launch) return 0;
   return mx_bytes(m, k) + mx_product_workspace(m, n, k);
+}
+
+std::string mx_linear_kernel(int64_t m, int64_t n, int64_t k, const std::string& dtype) {
+  check_product(m, n, k, n);
+  const char* names[] = {"", "way1", "way4", "way8", "way8x2"};
+  const Way way = way_of(m, n, k, size_of(type_of(dtype, "mx_linear: dtype must be bf16|f16|f32")));
+  return way == Way::launch ? mx_product_kernel(m, n, k) : names[static_cast<int>(way)];
 }
 
 void launch_mx_linear(int dev, const void* x, const std::string& dtype, int64_t x_stride, const void* w_codes,
@@ -782,7 +803,8 @@ void launch_mx_linear(int dev, const void* x, const std::string& dtype, int64_t 
   require(x && w_codes && w_scales && y, "mx_linear: null pointer");
   require(aligned(x, size_of(t)) && aligned(y, size_of(t)) && aligned(w_codes, 16) && aligned(w_scales, 16),
           "mx_linear: x and y aligned to their type, codes and scales to 16 bytes");
-  if (quantise_on_the_way(m, n, k, size_of(t))) {
+  const Way way = way_of(m, n, k, size_of(t));
+  if (way != Way::launch) {
     OnDevice on(dev);
     auto s = static_cast<hipStream_t>(stream);
     const Operand w = operand(w_codes, w_scales);
@@ -792,9 +814,9 @@ void launch_mx_linear(int dev, const void* x, const std::string& dtype, int64_t 
       auto out = static_cast<T*>(y);
       const auto rows = static_cast<unsigned>(m);
       const int len = static_cast<int>(k);
-      if (m == 1) few_rows<T, 1, 1, 2>(PlainRows<T, 1>{px, x_stride, rows, len}, w, m, n, k, out, y_stride, s);
-      else if (m <= 4) few_rows<T, 1, 1, 2>(PlainRows<T, 4>{px, x_stride, rows, len}, w, m, n, k, out, y_stride, s);
-      else if (n <= 16 * kComputeUnits) few_rows<T, 1, 1, 1>(PlainRows<T, 8>{px, x_stride, rows, len}, w, m, n, k, out, y_stride, s);
+      if (way == Way::one) few_rows<T, 1, 1, 2>(PlainRows<T, 1>{px, x_stride, rows, len}, w, m, n, k, out, y_stride, s);
+      else if (way == Way::four) few_rows<T, 1, 1, 2>(PlainRows<T, 4>{px, x_stride, rows, len}, w, m, n, k, out, y_stride, s);
+      else if (way == Way::eight) few_rows<T, 1, 1, 1>(PlainRows<T, 8>{px, x_stride, rows, len}, w, m, n, k, out, y_stride, s);
       else few_rows<T, 1, 2, 1>(PlainRows<T, 8>{px, x_stride, rows, len}, w, m, n, k, out, y_stride, s);
     });
     check(hipGetLastError(), "mx_linear");
