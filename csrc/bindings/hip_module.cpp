@@ -112,6 +112,7 @@ PYBIND11_MODULE(_hip, m) {
      py::arg("w_stride"), py::arg("m"), py::arg("n"), py::arg("k"), py::arg("y"), py::arg("y_stride"),
      py::arg("saved"), py::arg("saved_bytes"), py::arg("workspace"), py::arg("workspace_bytes"), py::arg("stream") = 0);
   m.def("mx_linear_grad_workspace", &mx_linear_grad_workspace, py::arg("m"), py::arg("n"), py::arg("k"));
+  m.def("mx_linear_grad_kernel", &mx_linear_grad_kernel, py::arg("m"), py::arg("n"), py::arg("k"));
   m.def("mx_linear_grad", [](int dev, uintptr_t dy, const std::string& dtype, int64_t dy_stride, uintptr_t saved,
                              int64_t m, int64_t n, int64_t k, uintptr_t dx, int64_t dx_stride, uintptr_t dw,
                              const std::string& w_dtype, int64_t dw_stride, uintptr_t workspace, size_t workspace_bytes,

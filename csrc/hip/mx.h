@@ -76,7 +76,10 @@ void launch_mx_linear_train(int dev, const void* x, const std::string& dtype, in
                             const std::string& w_dtype, int64_t w_stride, int64_t m, int64_t n, int64_t k, void* y,
                             int64_t y_stride, void* saved, size_t saved_bytes, void* workspace, size_t workspace_bytes,
                             void* stream);
+// A gradient has the same bits whether the other is asked for or not.
 size_t mx_linear_grad_workspace(int64_t m, int64_t n, int64_t k);
+// The tile that both gradients of one type take in one launch, or "" where each has its own (mx_product_kernel).
+std::string mx_linear_grad_kernel(int64_t m, int64_t n, int64_t k);
 void launch_mx_linear_grad(int dev, const void* dy, const std::string& dtype, int64_t dy_stride, const void* saved,
                            int64_t m, int64_t n, int64_t k, void* dx, int64_t dx_stride, void* dw,
                            const std::string& w_dtype, int64_t dw_stride, void* workspace, size_t workspace_bytes,

@@ -302,7 +302,7 @@ def linear_train(x, w):
 def linear_grad(dy, saved: LinearSaved, need_dx: bool = True, need_dw: bool = True):
     """Backward pass: ``(dx, dw)`` in x's and w's type (None where not needed). Straight-through: the
     gradients of the layer as if quantising were the identity, each product in 4 bits with dy
-    quantised along the axis that it contracts over."""
+    quantised along the axis that it contracts over. Neither's bits depend on whether the other is needed."""
     _check(dy, "dy")
     if not isinstance(saved, LinearSaved):
         raise TypeError(f"mx: saved must come from linear_train, not {type(saved).__name__}")

@@ -77,6 +77,18 @@ def test_no_kernel_is_without_a_size(H):
         assert name in PRODUCTS or name in LINEARS, (m, n, k)
 
 
+TRAININGS = {  # the tile of both gradients' launch, "" for a launch each
+    "64x64": [(631, 62, 2101)], "64x128": [(75, 73, 7890), (40, 520, 9000)], "128x128": [(1098, 65, 8181)],
+    "256x128": [(3534, 129, 8504)], "256x256": [(1166, 1203, 6308)], "": [(2449, 8475, 6300)],
+}
+
+
+def test_training_sizes_take_the_kernel_they_stand_for(H):
+    for name, sizes in TRAININGS.items():
+        for size in sizes:
+            assert H.mx_linear_grad_kernel(*size) == name, size
+
+
 def whole(rows, k, seed):
     g = torch.Generator(device="cuda").manual_seed(seed)
     grid = torch.tensor([0, 1, 2, 3, 4, 6, -1, -2, -3, -4, -6.0], device="cuda")
@@ -110,11 +122,10 @@ def test_linear_layers_of_whole_numbers(name, size):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("m,n,k", [(75, 73, 7890), (631, 62, 2101), (1098, 65, 8181), (3534, 129, 8504), (1166, 1203, 6308),
-                                   (40, 520, 9000), (2449, 8475, 6300)])
+@pytest.mark.parametrize("m,n,k", [s for sizes in TRAININGS.values() for s in sizes])
 @pytest.mark.parametrize("dtype,w_dtype", [(BF16, BF16), (F16, F16), (F32, F32), (F16, F32)])
 def test_training_steps_of_whole_numbers(m, n, k, dtype, w_dtype):
-    """Gradients in one launch by tiles of every size, and each in its own (other types, and the last sizes)."""
+    """Gradients in one launch by tiles of every size, and each in its own (other types, and the last size)."""
     from gpumon.ops import mx
 
     x, w, dy = whole(m, k, 1), whole(n, k, 2), whole(m, n, 3)
