@@ -140,8 +140,8 @@ class MxTensor:
     def parts(self):
         """(codes, scales) row-major, as :meth:`pack` takes them."""
         blocks, r16 = -(-self.k // BLOCK), -(-self.rows // 16) * 16
-        codes = self.codes.permute(0, 3, 1, 2, 4).reshape(r16, -1)[:self.rows, :blocks * 16]
-        scales = self.scales.permute(0, 3, 1, 4, 2).reshape(r16, -1)[:self.rows, :blocks]
+        codes = self.codes.permute(0, 3, 1, 2, 4).reshape(r16, -(-self.k // 128) * 64)[:self.rows, :blocks * 16]
+        scales = self.scales.permute(0, 3, 1, 4, 2).reshape(r16, -(-self.k // 512) * 16)[:self.rows, :blocks]
         return codes.contiguous(), scales.contiguous()
 
     def record_stream(self, stream) -> None:
