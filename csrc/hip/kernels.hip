@@ -28,8 +28,10 @@ static int64_t mono_ns() {
 }
 
 void check(int err, const char* what) {
-  if (err != hipSuccess)
+  if (err != hipSuccess) {
+    (void)hipGetLastError();  // reported here: the thread's next check, ours or another library's, is not to find it
     throw std::runtime_error(std::string(what) + ": " + hipGetErrorString(static_cast<hipError_t>(err)));
+  }
 }
 
 int device_count() {
