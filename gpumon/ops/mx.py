@@ -16,8 +16,10 @@ nearest, halves to the even code, and end at 6. A block with a NaN or an infinit
 
 Tensors are bf16, f16 or f32 on one GPU; work goes to that device's current torch stream and can be
 captured into a graph (workspaces come from torch's allocator, so each graph has its own). Results
-carry no autograd graph: :func:`linear_grad` is the backward pass. Errors of arguments are
-``ValueError`` / ``TypeError``, before anything is launched.
+carry no autograd graph: :func:`linear_grad` is the backward pass, and where a gradient would be lost
+(an input of the linear layer that requires one while they are recorded, or has a tangent) the call is
+refused; under ``torch.no_grad()``, as in the forward pass of a ``torch.autograd.Function``, it is not.
+Errors of arguments are ``ValueError`` / ``TypeError``, before anything is launched.
 """
 
 from __future__ import annotations
@@ -25,6 +27,7 @@ from __future__ import annotations
 import functools
 
 import torch
+from torch.autograd import forward_ad
 
 from .._native import hip as _load_hip
 
@@ -54,6 +57,14 @@ def _check(t, name: str, ndim=None):
     if t.dtype not in DTYPES:
         raise TypeError(f"mx: {name} is {t.dtype}: one of bfloat16, float16, float32")
     raise ValueError(f"mx: {name} has {t.dim()} dimensions, expected {ndim}")
+
+
+def _check_constant(t, name: str):
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"mx: {name} requires a gradient, which the result would not carry: detach it, or call under "
+                         "torch.no_grad() and take linear_train's gradients from linear_grad")
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+        raise ValueError(f"mx: {name} has a tangent, which the result would not carry")
 
 
 def _check_dtype(dtype):
@@ -238,6 +249,7 @@ def matmul(a: MxTensor, b: MxTensor, dtype=torch.bfloat16):
 def linear(x, w: MxTensor):
     """x [..., k] on weights w (n x k): x quantised along k, times w.T; [..., n] in x's type."""
     _check(x, "x")
+    _check_constant(x, "x")
     _check_mx(w, "w")
     if x.dim() < 1 or x.shape[-1] != w.k:
         raise ValueError(f"mx: x is {tuple(x.shape)}, its last size must be the weights' k = {w.k}")
@@ -272,6 +284,8 @@ def linear_train(x, w):
     """Forward pass with x [..., k] and w [n, k] both quantised here: ``(y [..., n], saved)``."""
     _check(x, "x")
     _check(w, "w", 2)
+    _check_constant(x, "x")
+    _check_constant(w, "w")
     if x.dim() < 1 or x.shape[-1] != w.shape[1]:
         raise ValueError(f"mx: x is {tuple(x.shape)}, w {tuple(w.shape)}: the last sizes differ")
     if x.device != w.device:
@@ -304,6 +318,7 @@ def linear_grad(dy, saved: LinearSaved, need_dx: bool = True, need_dw: bool = Tr
     gradients of the layer as if quantising were the identity, each product in 4 bits with dy
     quantised along the axis that it contracts over. Neither's bits depend on whether the other is needed."""
     _check(dy, "dy")
+    _check_constant(dy, "dy")
     if not isinstance(saved, LinearSaved):
         raise TypeError(f"mx: saved must come from linear_train, not {type(saved).__name__}")
     m, n, k, dev = saved.rows, saved.n, saved.k, saved.device
