@@ -15,17 +15,15 @@ namespace mx {
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
-typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
 // The conversions of gfx950 divide (multiply) by the scale's power of two exactly, round halves to
-// even and saturate at 6, for every scale byte 0..254 including 2^-127, and read 255 as NaN; checked
-// over all 16-bit inputs times all scales against the definition.
+// even and saturate at 6, for every scale byte 0..254 including 2^-127, and read 255 as NaN; tested
+// over all 16-bit inputs under all scales that they can have, and back over all codes times all scales.
 __device__ __forceinline__ float scale_of(unsigned byte) { return __builtin_bit_cast(float, byte << 23); }
 
 // Scale byte of a block from the bits of its largest magnitude as an f32 (magnitudes order like their
@@ -41,7 +39,6 @@ struct Elem;
 template <>
 struct Elem<__bf16> {
   static constexpr int kPerWord = 2;
-  using Word = unsigned;  // two elements
   __device__ static unsigned amax(unsigned m, unsigned w) {  // running magnitudes, per half
     return __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(u16x2, m),
                                                                   __builtin_bit_cast(u16x2, w & 0x7fff7fffu)));
@@ -56,7 +53,6 @@ struct Elem<__bf16> {
 template <>
 struct Elem<_Float16> {
   static constexpr int kPerWord = 2;
-  using Word = unsigned;
   __device__ static unsigned amax(unsigned m, unsigned w) { return Elem<__bf16>::amax(m, w); }
   __device__ static unsigned amax_f32(unsigned m) {
     const unsigned h = max(m >> 16, m & 0xffffu);  // an infinity or NaN converts to one
@@ -71,7 +67,6 @@ struct Elem<_Float16> {
 template <>
 struct Elem<float> {
   static constexpr int kPerWord = 1;
-  using Word = unsigned;
   __device__ static unsigned amax(unsigned m, unsigned w) { return max(m, w & 0x7fffffffu); }
   __device__ static unsigned amax_f32(unsigned m) { return m; }
   template <int SEL>

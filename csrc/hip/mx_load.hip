@@ -14,7 +14,8 @@ int64_t now_ns() {
   return std::chrono::duration_cast<std::chrono::nanoseconds>(std::chrono::steady_clock::now().time_since_epoch()).count();
 }
 
-// bf16 values near a normal distribution: the sum of four uniform ones from a hash of the index.
+// bf16 values near a normal distribution: the sum of four uniform ones from a hash of the index (the published
+// 64-bit mixer splitmix64).
 __global__ void __launch_bounds__(256) random_kernel(__bf16* x, size_t n, uint32_t seed) {
   for (size_t i = blockIdx.x * size_t{256} + threadIdx.x; i < n; i += size_t{256} * gridDim.x) {
     uint64_t h = (i + 1) * 0x9e3779b97f4a7c15ull + seed;

@@ -3,7 +3,7 @@
 What a node that serves or trains in 4 bits runs on the matrix path that
 ``gpu_mfma_tflops{dtype="f6f4"}`` counts, as hand-written gfx950 kernels (``csrc/hip/mx_quant.hip``,
 ``csrc/hip/mx_product.hip``; format and layout: ``csrc/hip/mx.h``). ``gpumon load --kind mxlinear``
-drives the card with them.
+drives the card with the linear layer on quantised weights; the training step is for programs that call it.
 
 An MXFP4 matrix holds 32 consecutive elements of a row as 4-bit numbers (0, 0.5, 1, 1.5, 2, 3, 4, 6
 and their negatives) times one power of two, ``2^(floor(log2 amax) - 2)``; elements are rounded to
