@@ -31,7 +31,8 @@ inline int64_t mx_codes_bytes(int64_t rows, int64_t k) { return mx_row_blocks(ro
 inline int64_t mx_scales_bytes(int64_t rows, int64_t k) { return mx_row_blocks(rows) * mx_groups(k) * 256; }
 // Limits of the kernels' indexes and grids: 2^24 pieces of 16 rows x 512 elements (more than fits the
 // card in 16 bits an element) and 2^28 elements along a row (a row block's offsets stay within 32
-// bits); a product also has at most 2^28 pieces of 16 x 16 results.
+// bits); a product also has at most 2^28 pieces of 16 x 16 results, and quantising down the columns fewer
+// than 2^23 tiles of 32 x 512 in a launch.
 inline bool mx_fits(int64_t rows, int64_t k) {
   return rows < (1ll << 28) && k <= (1ll << 28) && mx_row_blocks(rows) * mx_groups(k) < (1ll << 24);
 }

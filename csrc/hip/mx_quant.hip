@@ -228,34 +228,50 @@ void check_matrix(const void* data, int64_t rows, int64_t k, int64_t stride, con
 
 unsigned blocks_for(int64_t n, int64_t per) { return static_cast<unsigned>((n + per - 1) / per); }
 
+unsigned tiles_of(const Both* of, int count) { return of[0].blocks + (count > 1 ? of[1].blocks : 0); }
+
 template <typename T, bool ROWS>
 void launch_tiles(const Both* of, int count, hipStream_t s) {
-  TwoBoth both{{of[0], of[count - 1]}};
-  for (Both& m : both.of) m.blocks = static_cast<unsigned>(mx_quads(m.rows) * 4) * m.groups.d;
-  hipLaunchKernelGGL((quantize_tile_kernel<T, ROWS>), dim3(both.of[0].blocks + (count > 1 ? both.of[1].blocks : 0)), dim3(512),
-                     0, s, both);
+  const TwoBoth both{{of[0], of[count - 1]}};
+  hipLaunchKernelGGL((quantize_tile_kernel<T, ROWS>), dim3(tiles_of(of, count)), dim3(512), 0, s, both);
 }
 Both both_of(const void* x, int64_t rows, int64_t k, int64_t stride, void* rc, void* rs, void* cc, void* cs) {
-  return {x, stride, static_cast<unsigned>(rows), static_cast<int>(k), Div(static_cast<unsigned>(mx_groups(k))), 0,
+  const unsigned groups = static_cast<unsigned>(mx_groups(k));
+  return {x, stride, static_cast<unsigned>(rows), static_cast<int>(k), Div(groups), static_cast<unsigned>(mx_quads(rows) * 4) * groups,
           static_cast<char*>(rc), static_cast<char*>(rs), static_cast<char*>(cc), static_cast<char*>(cs)};
+}
+// A launch has fewer than 2^32 threads.
+bool fits_launch(int64_t rows, int64_t k) { return mx_quads(rows) * 4 * mx_groups(k) < (1ll << 23); }
+void check_both(const void* x, int64_t rows, int64_t k, int64_t stride, const void* row_codes, const void* row_scales,
+                const void* col_codes, const void* col_scales, Type t) {
+  check_matrix(x, rows, k, stride, row_codes, row_scales, t);
+  require(rows >= 1, "mx: down the columns, rows must be >= 1");
+  check_matrix(x, k, rows, rows, col_codes, col_scales, t);
+  require(fits_launch(rows, k), "mx: rows and k are beyond the limits (mx.h)");
 }
 
 }  // namespace
 
 void check_source(const Source& s, Type t) {
-  check_matrix(s.x, s.rows, s.k, s.stride, s.along, s.along, t);
-  require(s.rows >= 1, "mx: rows must be >= 1");
-  check_matrix(s.x, s.k, s.rows, s.rows, s.down, s.down, t);
+  check_both(s.x, s.rows, s.k, s.stride, s.along, s.along, s.down, s.down, t);
 }
 void launch_quantize_both(int dev, const Source* sources, int count, Type t, hipStream_t s) {
-  OnDevice on(dev);
   Both of[2];
   for (int i = 0; i < count; ++i) {
     const Source& m = sources[i];
     const Quantized along{m.along, m.rows, m.k}, down{m.down, m.k, m.rows};
     of[i] = both_of(m.x, m.rows, m.k, m.stride, along.at, along.scales(), down.at, down.scales());
   }
-  with_type(t, [&](auto e) { launch_tiles<decltype(e), true>(of, count, s); });
+  OnDevice on(dev);
+  with_type(t, [&](auto e) {
+    using T = decltype(e);
+    if (count == 2 && tiles_of(of, 2) >= 1u << 23) {
+      launch_tiles<T, true>(of, 1, s);
+      launch_tiles<T, true>(of + 1, 1, s);
+    } else {
+      launch_tiles<T, true>(of, count, s);
+    }
+  });
   check(hipGetLastError(), "mx_quantize_both");
 }
 
@@ -266,15 +282,12 @@ using namespace mx;
 void launch_mx_quantize(int dev, const void* x, const std::string& dtype, int64_t rows, int64_t k, int64_t stride,
                         bool by_column, void* codes, void* scales, void* stream) {
   const Type t = type_of(dtype, "mx_quantize: dtype must be bf16|f16|f32");
-  check_matrix(x, rows, k, stride, codes, scales, t);
-  if (by_column) {
-    require(rows >= 1, "mx_quantize: by column, rows must be >= 1");
-    check_matrix(x, k, rows, rows, codes, scales, t);
-  }
+  if (by_column) check_both(x, rows, k, stride, codes, scales, codes, scales, t);
+  else check_matrix(x, rows, k, stride, codes, scales, t);
   if (rows == 0) return;
-  OnDevice on(dev);
   auto s = static_cast<hipStream_t>(stream);
   auto pc = static_cast<char*>(codes), ps = static_cast<char*>(scales);
+  OnDevice on(dev);
   with_type(t, [&](auto e) {
     using T = decltype(e);
     auto px = static_cast<const T*>(x);
@@ -294,9 +307,7 @@ void launch_mx_quantize(int dev, const void* x, const std::string& dtype, int64_
 void launch_mx_quantize_both(int dev, const void* x, const std::string& dtype, int64_t rows, int64_t k, int64_t stride,
                              void* row_codes, void* row_scales, void* col_codes, void* col_scales, void* stream) {
   const Type t = type_of(dtype, "mx_quantize_both: dtype must be bf16|f16|f32");
-  check_matrix(x, rows, k, stride, row_codes, row_scales, t);
-  require(rows >= 1, "mx_quantize_both: rows must be >= 1");
-  check_matrix(x, k, rows, rows, col_codes, col_scales, t);
+  check_both(x, rows, k, stride, row_codes, row_scales, col_codes, col_scales, t);
   OnDevice on(dev);
   const Both of = both_of(x, rows, k, stride, row_codes, row_scales, col_codes, col_scales);
   with_type(t, [&](auto e) { launch_tiles<decltype(e), true>(&of, 1, static_cast<hipStream_t>(stream)); });
