@@ -91,10 +91,11 @@ __device__ __forceinline__ void hold() {
 //
 // The larger the tile the less each element is read: 256 x 256 results need 32 KiB a stage for 64 matrix
 // instructions a SIMD. Eight waves of 128 x 64, since four of 128 x 128, which read a third less from LDS,
-// were no faster (8192^3 236 to 254 us, these 240 to 261). What bounds large products is most likely the
-// power their operands' bits take: the same launch takes 212 to 261 us on random ones (5.2 to 4.2 PFLOP/s)
-// and 157 to 167 on zeros; matrix instructions alone, on random registers, come to 7.25 PFLOP/s. About 10
-// us of a launch are its first loads and last stores (one tile a compute unit, fitted over k). Smaller
+// were no faster (8192^3 236 to 254 us, these 240 to 261 in the same run). What bounds large products is the
+// power their operands' bits take: for seconds on end 8192^3 takes 223 us on random ones, 1379 to 1393 W of the
+// card's 1400 at 1692 MHz, and 157 on zeros, 1100 W at 2384 MHz; over runs and cards 212 to 261 and 157 to 174.
+// Matrix instructions alone, on random registers, come to 7.10 PFLOP/s, and 6.49 in the 32x32x64 form. About
+// 10 us of a launch are its first loads and last stores (one tile a compute unit, fitted over k). Smaller
 // tiles are for fewer results, so that every compute unit has one (kTiles has what each takes).
 //
 // One launch takes up to two products, the second's tiles after the first's.

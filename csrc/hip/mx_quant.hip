@@ -44,7 +44,7 @@ struct Piece {
 // Blocks along a row: amax, the scale's exponent and the codes as in mx.h. A wave takes 512 elements of four
 // rows, their loads in flight together; a workgroup ends up with whole chunks and scale words and writes
 // them 16 bytes a lane. Bound by memory: 8192 x 8192 bf16 (134 MB read, 36 written) 28.7 us, 5.9 TB/s,
-// where a plain copy of 1 GiB reaches 6.55; one token of 8192 2.8 us, a launch's least.
+// where a plain copy of 1 GiB reaches 6.54; one token of 8192 2.8 us, a launch's least.
 template <typename T>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const T* __restrict__ x, int64_t stride, unsigned rows,
                                                             int k, Div groups, unsigned quads, char* __restrict__ codes,
